@@ -435,6 +435,60 @@ int netra_moe_sort_static_scratch_launch(const int32_t* topk_ids_i32, int32_t* p
                                          int32_t* inv_perm_i32, int32_t* counts_i32,
                                          int32_t* offsets_i32, uint32_t rows, cudaStream_t stream);
 
+/* ------------------------------------------------------------------ dense block-scaled FP8 linear map
+ * The operation of the compiler's dense contract (compiler/netra_compiler/contracts.py:175-284), at any size.
+ * Element types: 0 = BF16, 1 = FP16, 2 = FP32.  Pitches are in elements.  Weights are E4M3 codes [w_rows, w_cols],
+ * row-major, with one FP32 scale per 128 x 128 block, [ceil(w_rows/128)] rows of w_scale_pitch >= ceil(w_cols/128).
+ * Codes need 16-byte aligned addresses and row pitches; nothing else has an alignment beyond its element.  Sizes are
+ * 1..2^26.  Nothing is allocated, synchronised or kept between calls; every call may be captured. */
+
+/* scale[m,b] = max(amax |x[m, 128 columns of block b]|, 1e-10) * fl(1/448), codes = e4m3_rne_sat(x * fl(1/scale)), all in
+ * FP32: the layer's own quantiser.  The scale of (m, b) goes to scale_f32[m * scale_row_stride + b * scale_block_stride].
+ * An infinity makes its block's scale infinite; a NaN stays at its element. */
+int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, float* scale_f32, uint64_t scale_row_stride,
+                                     uint64_t scale_block_stride, const void* x, uint32_t x_dtype, uint64_t x_pitch,
+                                     uint32_t m, uint32_t k, cudaStream_t stream);
+
+/* out[m, n] = sum over K-blocks b of a_scale[m,b] * w_scale[.,.] * sum_{k in b} a[m,k] * w, FP32, blocks ascending, one
+ * rounding to out_dtype.  transpose_w = 0: w is [n, k] (a linear layer's weight); 1: w is [k, n] as stored (the gradient to
+ * a linear layer's input: w_rows is the reduction).  Scale strides as above. */
+int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pitch, const void* a_fp8, uint64_t a_pitch,
+                                  const float* a_scale_f32, uint64_t a_scale_row_stride, uint64_t a_scale_block_stride,
+                                  const void* w_fp8, uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch,
+                                  uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols, cudaStream_t stream);
+
+/* Both in one call: quantises the rows of x into the workspace and multiplies; out has x's type.  The workspace is 16-byte
+ * aligned device memory of netra_dense_fp8_linear_workspace_bytes(m, reduction length) bytes, free again when the
+ * call's work is done on the stream. */
+uint64_t netra_dense_fp8_linear_workspace_bytes(uint32_t m, uint32_t k);
+int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, uint32_t dtype, uint64_t x_pitch,
+                                  const void* w_fp8, uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch,
+                                  uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols, void* workspace,
+                                  uint64_t workspace_bytes, cudaStream_t stream);
+
+/* The current device's status words of the dense kernels (synchronises): word 0 is 0, or the role whose bounded wait ran out. */
+int netra_dense_status(uint32_t status_out[4]);
+
+/* ------------------------------------------------------------------ router load and balance loss
+ * counts[e] = number of (token, slot) pairs of counted tokens whose id is e.  ids are i32 or i64 (id_bytes 4 or 8), rows
+ * id_pitch elements apart; ids outside 0..experts-1 (padding, the shared slot) are not counted.  token_mask: one byte per
+ * token, 0 = not counted; NULL counts all.  experts is 1..1024. */
+int netra_expert_counts_launch(int32_t* counts_i32, const void* ids, uint32_t id_bytes, uint64_t id_pitch,
+                               const uint8_t* token_mask, uint64_t tokens, uint32_t slots, uint32_t experts,
+                               cudaStream_t stream);
+
+/* With f = counts / sum counts, p_t = softmax(logits_t) and n counted tokens:
+ *   loss = experts / n * sum_t sum_e f_e p_te          grad_te = upstream * experts / n * p_te * (f_e - sum_j f_j p_tj)
+ * scale_f32 receives experts / n, which the gradient reads.  No counted token, or no count: 0.  A row without a finite logit counts as a token and contributes 0; rows not counted are not read and get
+ * a zero gradient.  The workspace (16-byte aligned) is free again when the call's work is done on the stream. */
+uint64_t netra_balance_loss_workspace_bytes(void);
+int netra_balance_loss_launch(float* loss_f32, float* scale_f32, const void* logits, uint32_t dtype, uint64_t pitch,
+                              const int32_t* counts_i32, const uint8_t* token_mask, void* workspace,
+                              uint64_t workspace_bytes, uint64_t tokens, uint32_t experts, cudaStream_t stream);
+int netra_balance_loss_grad_launch(void* grad, uint64_t grad_pitch, const void* logits, uint32_t dtype, uint64_t pitch,
+                                   const int32_t* counts_i32, const uint8_t* token_mask, const float* scale_f32,
+                                   const float* upstream_f32, uint64_t tokens, uint32_t experts, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -106,6 +106,18 @@ SIGNATURES = {
     "netra_moe_layer_destroy": (c_int, [c_void_p]),
     "netra_moe_last_error": (ctypes.c_char_p, []),
     "netra_moe_sort_static_scratch_launch": (c_int, [c_void_p] * 5 + [c_u32, c_void_p]),
+    "netra_dense_quantize_rows_launch": (c_int, [c_void_p, c_u64, c_void_p, c_u64, c_u64, c_void_p, c_u32, c_u64, c_u32, c_u32, c_void_p]),
+    "netra_dense_fp8_matmul_launch": (c_int, [c_void_p, c_u32, c_u64, c_void_p, c_u64, c_void_p, c_u64, c_u64, c_void_p, c_u64, c_void_p,
+                                              c_u64, c_u32, c_u32, c_u32, c_u32, c_void_p]),
+    "netra_dense_fp8_linear_workspace_bytes": (c_u64, [c_u32, c_u32]),
+    "netra_dense_fp8_linear_launch": (c_int, [c_void_p, c_u64, c_void_p, c_u32, c_u64, c_void_p, c_u64, c_void_p, c_u64, c_u32, c_u32,
+                                              c_u32, c_u32, c_void_p, c_u64, c_void_p]),
+    "netra_dense_status": (c_int, [ctypes.POINTER(c_u32 * 4)]),
+    "netra_expert_counts_launch": (c_int, [c_void_p, c_void_p, c_u32, c_u64, c_void_p, c_u64, c_u32, c_u32, c_void_p]),
+    "netra_balance_loss_workspace_bytes": (c_u64, []),
+    "netra_balance_loss_launch": (c_int, [c_void_p, c_void_p, c_void_p, c_u32, c_u64, c_void_p, c_void_p, c_void_p, c_u64, c_u64, c_u32, c_void_p]),
+    "netra_balance_loss_grad_launch": (c_int, [c_void_p, c_u64, c_void_p, c_u32, c_u64, c_void_p, c_void_p, c_void_p, c_void_p, c_u64,
+                                               c_u32, c_void_p]),
 }
 for _b in BRIDGES:
     SIGNATURES[_b + "_load"] = (c_int, [ctypes.c_char_p])

@@ -826,3 +826,7 @@ int netra_moe_layer_destroy(netra_moe_layer_t* layer) {
 
 // The reference's 768-row prefill bridge on this library's stages (needs launch_stage() from above).
 #include "prefill_m768_bridge.cu"
+
+// The dense block-scaled FP8 linear map with its row quantiser, and the router's balance loss (need the helpers from above).
+#include "dense_fp8.cu"
+#include "balance.cu"

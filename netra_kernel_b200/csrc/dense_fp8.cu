@@ -1,0 +1,416 @@
+// The dense block-scaled FP8 linear map, the operation the compiler's dense contract names
+// (compiler/netra_compiler/contracts.py:175-284): E4M3 codes with one FP32 scale per row and 128 columns on the left, per
+// 128 x 128 block on the right, FP32 accumulation, K-blocks ascending.
+//
+//   quantise   s[m,b] = max(amax |x[m, block b]|, 1e-10) * fl(1/448),  a = e4m3_rne_sat(x * fl(1/s))      (the layer's quantiser)
+//   product    y[m,n] = sum_b  sa[m,b] * sw[n/128,b] * sum_{k in b} a[m,k] w[n,k]
+//   gradient   dx[m,k] = sum_b sg[m,b] * sw[b,k/128] * sum_{n in b} g[m,n] w[n,k]      (w read as it is stored)
+//
+// Any M, N, K: codes need 16-byte row pitches (TMA), everything else is masked.
+#include <type_traits>
+
+namespace netra {
+
+enum : uint32_t { kDenseBf16 = 0, kDenseF16 = 1, kDenseF32 = 2 };
+
+// Where a bounded wait of a dense kernel ran out (kStatus* codes); read by netra_dense_status.
+__device__ uint32_t g_dense_status[4];
+
+__device__ __forceinline__ float dense_load(const void* p, uint32_t dtype, size_t i) {
+  if (dtype == kDenseBf16) return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+  if (dtype == kDenseF16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
+  return reinterpret_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void dense_store(void* p, uint32_t dtype, size_t i, float v) {
+  if (dtype == kDenseBf16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else if (dtype == kDenseF16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  else reinterpret_cast<float*>(p)[i] = v;
+}
+
+// ------------------------------------------------------------------------------------------
+// Row quantiser.  Sixteen lanes own one block of 128 columns, eight neighbouring columns each.
+// Scales go to scale[m * scale_row + b * scale_block].
+// ------------------------------------------------------------------------------------------
+extern "C" __global__ void __launch_bounds__(256)
+netra_dense_quantize_rows_sm100(const void* __restrict__ x, uint32_t dtype, uint64_t x_pitch, uint8_t* __restrict__ codes,
+                                uint64_t codes_pitch, float* __restrict__ scale, uint64_t scale_row, uint64_t scale_block,
+                                uint32_t m, uint32_t k) {
+  const uint32_t blocks = (k + kBlock - 1) / kBlock;
+  const uint64_t total = (uint64_t)m * blocks;
+  const int sub = threadIdx.x & 15;
+  const uint64_t item = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+  const bool live = item < total;
+  const uint64_t row = live ? item / blocks : 0;
+  const uint32_t b = live ? (uint32_t)(item - row * blocks) : 0;
+  float v[8];
+  float amax = amax_floor();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t col = b * kBlock + sub * 8 + j;
+    v[j] = live && col < k ? dense_load(x, dtype, row * x_pitch + col) : 0.0f;
+    amax = fmaxf(amax, fabsf(v[j]));
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  if (!live) return;
+  const float s = amax * inv448();
+  const float inv = 1.0f / s;
+  if (sub == 0) scale[row * scale_row + b * scale_block] = s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t col = b * kBlock + sub * 8 + j;
+    if (col < k) codes[row * codes_pitch + col] = f32_to_e4m3(v[j] * inv);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Product on the tensor cores.  A cluster owns 128 rows x kBN columns of the output and splits the K-blocks among
+// its CTAs; per K-block the raw sums leave TMEM and are promoted as acc = fma(part, sa * sw, acc), as in the grouped GEMMs.
+//   warp 0: TMA producer, warp 1: MMA issuer (owns TMEM), warps 4..11: promotion (two groups halve the columns)
+// At the end every CTA lays its FP32 partial tile into its shared memory and sums a share of the rows over the cluster
+// in rank order (deterministic).
+// ------------------------------------------------------------------------------------------
+constexpr int kDnThreads = 384;
+
+template <int kBN>
+struct DnCfg {
+  static constexpr int kABytes = 128 * kBlock;
+  static constexpr int kBBytes = kBN * kBlock;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = kBN >= 128 ? 6 : 8;
+  static constexpr int kAccStages = 512 / kBN > 4 ? 4 : 512 / kBN;
+  static constexpr int kTmemCols = kAccStages * kBN;
+  static constexpr int kOutPitch = kBN + 4;            // floats; 16-byte row stores fall on different banks
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512;
+  static_assert(128 * kOutPitch * 4 <= kStages * kStageBytes, "the partial tile reuses the stages");
+  static_assert(kSmemBytes <= 232448, "exceeds the shared memory of one SM");
+};
+
+struct DnArgs {
+  const float* a_scale;
+  uint64_t a_scale_row, a_scale_block;
+  const float* w_scale;
+  uint64_t w_scale_col, w_scale_block;    // per 128 output columns, per K-block
+  void* out;
+  uint64_t out_pitch;
+  uint32_t out_dtype;
+  uint32_t m, n, k_blocks;                // rows, output columns, K-blocks
+  uint32_t n_tiles;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
+}
+
+// MN-major, 128-byte-swizzled operand tile: 128 output columns (bytes) per row, one row per reduction index; groups of
+// eight rows are 1,024 bytes apart.
+__device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t addr) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// kTransposed: the weight tile is [128 reduction rows][128 output columns] as stored, an MN-major B operand.
+template <int kBN, bool kTransposed>
+__global__ void __launch_bounds__(kDnThreads, 1)
+netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w, const DnArgs g) {
+  using C = DnCfg<kBN>;
+  static_assert(!kTransposed || kBN == 128, "a transposed weight tile is one 128-byte swizzle atom wide");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = full_bar + C::kStages;
+  uint64_t* tfull_bar = empty_bar + C::kStages;
+  uint64_t* tempty_bar = tfull_bar + C::kAccStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + C::kAccStages);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const uint32_t tile = blockIdx.x / ranks;
+  const uint32_t row0 = (tile / g.n_tiles) * 128u, col0 = (tile % g.n_tiles) * (uint32_t)kBN;
+  const uint32_t kb0 = (uint32_t)((uint64_t)g.k_blocks * rank / ranks), kb1 = (uint32_t)((uint64_t)g.k_blocks * (rank + 1) / ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
+    for (int a = 0; a < C::kAccStages; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 8); }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    const uint64_t pol = policy_evict_last();
+    for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      const uint32_t it = kb - kb0, s = it % C::kStages;
+      if (!mbar_wait(smem_u32(&empty_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) { g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; break; }
+      const uint32_t bar = smem_u32(&full_bar[s]), dst = smem_u32(smem + s * C::kStageBytes);
+      mbar_expect_tx(bar, C::kStageBytes);
+      tma_load_2d(dst, &tm_a, bar, (int)(kb * kBlock), (int)row0, pol);
+      if (kTransposed) tma_load_2d(dst + C::kABytes, &tm_w, bar, (int)col0, (int)(kb * kBlock), pol);
+      else tma_load_2d(dst + C::kABytes, &tm_w, bar, (int)(kb * kBlock), (int)col0, pol);
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = make_idesc(kBN) | (kTransposed ? 1u << 16 : 0u);
+    for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      const uint32_t it = kb - kb0, s = it % C::kStages, a = it % C::kAccStages;
+      if (!mbar_wait(smem_u32(&tempty_bar[a]), ((it / C::kAccStages) & 1) ^ 1, abort_flag) ||
+          !mbar_wait(smem_u32(&full_bar[s]), (it / C::kStages) & 1, abort_flag)) { g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break; }
+      tc_fence_after();
+      const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
+      const uint64_t adesc = make_smem_desc(sa);
+      const uint64_t bdesc = kTransposed ? make_smem_desc_mn(sa + C::kABytes) : make_smem_desc(sa + C::kABytes);
+#pragma unroll
+      for (int k = 0; k < kBlock / 32; ++k)
+        umma_f8(tmem_base + a * kBN, adesc + 2 * k, bdesc + (kTransposed ? 256 : 2) * k, idesc, k > 0);
+      umma_commit(smem_u32(&empty_bar[s]));
+      umma_commit(smem_u32(&tfull_bar[a]));
+    }
+  } else if (warp >= 4) {
+    constexpr int kCols = kBN / 2;                      // columns of this thread
+    const int wg = (warp - 4) >> 2, quad = warp & 3;
+    const uint32_t r = (uint32_t)(quad * 32 + lane), row = row0 + r;
+    const float* sa_ptr = g.a_scale + (uint64_t)min(row, g.m - 1) * g.a_scale_row;
+    const float* sw_ptr = g.w_scale + (uint64_t)((col0 + wg * kCols) / kBlock) * g.w_scale_col;
+    if ((col0 + wg * kCols) >= g.n) sw_ptr = g.w_scale;         // columns past the end: nothing is stored
+    float acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
+    float sa = kb0 < kb1 ? __ldg(sa_ptr + kb0 * g.a_scale_block) : 0.0f, sw = kb0 < kb1 ? __ldg(sw_ptr + kb0 * g.w_scale_block) : 0.0f;
+    for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      const uint32_t it = kb - kb0, a = it % C::kAccStages;
+      const float s = __fmul_rn(sa, sw);
+      if (kb + 1 < kb1) { sa = __ldg(sa_ptr + (kb + 1) * g.a_scale_block); sw = __ldg(sw_ptr + (kb + 1) * g.w_scale_block); }
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (it / C::kAccStages) & 1, abort_flag))) { g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; break; }
+      tc_fence_after();
+      const uint32_t t = tmem_base + ((uint32_t)(quad * 32) << 16) + a * kBN + wg * kCols;
+      uint32_t v[kCols / 32][32];
+#pragma unroll
+      for (int q = 0; q < kCols / 32; ++q) tmem_ld32_nowait(t + 32 * q, v[q]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[a]));
+#pragma unroll
+      for (int q = 0; q < kCols / 32; ++q)
+#pragma unroll
+        for (int c = 0; c < 32; ++c) acc[32 * q + c] = fmaf(__uint_as_float(v[q][c]), s, acc[32 * q + c]);
+    }
+    __syncwarp();
+    // every MMA of this CTA has completed (the last accumulator stage was waited for), so the stages are free
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    float* dst = reinterpret_cast<float*>(smem) + (size_t)r * C::kOutPitch + wg * kCols;
+#pragma unroll
+    for (int c = 0; c < kCols; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) __nanosleep(200000);   // copies in flight land before the CTA goes on
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::kTmemCols);
+  }
+  __syncwarp();
+  if (ranks > 1) cluster_barrier();
+  // rows r = rank, rank + ranks, ... ; a warp takes a row, a lane four neighbouring columns at a time
+  const uint32_t base = smem_u32(smem);
+  for (uint32_t i = warp; i * ranks + rank < 128u; i += kDnThreads / 32) {
+    const uint32_t r = i * ranks + rank, row = row0 + r;
+    if (row >= g.m) break;
+    for (uint32_t c = lane * 4; c < (uint32_t)kBN; c += 128) {
+      if (col0 + c >= g.n) break;
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (uint32_t j = 0; j < ranks; ++j) {
+        const uint32_t addr = base + (r * C::kOutPitch + c) * 4;
+        const float4 p = ld_cluster_f4(addr, j);
+        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+      }
+      const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col0 + c + j < g.n) dense_store(g.out, g.out_dtype, (uint64_t)row * g.out_pitch + col0 + c + j, o[j]);
+    }
+  }
+  __syncwarp();
+  if (ranks > 1) cluster_barrier();            // nobody leaves while its partial tile is being read
+}
+
+}  // namespace netra
+
+namespace {
+
+// Byte tensor of `rows` rows of `cols` codes, `pitch` bytes apart; box 128 bytes x box_rows, 128-byte swizzle.
+int encode_codes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return fail("cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_error, sizeof g_error, "cuTensorMapEncodeTiled (FP8 codes) failed with CUresult %d", (int)r);
+    return -1;
+  }
+  return 0;
+}
+
+std::mutex g_dense_mutex;
+int g_dense_sms[kMaxDevices] = {};      // SM count once the kernels of a device are set up
+
+int dense_setup(int* sms) {
+  int device = 0;
+  if (int rc = current_device_index(&device)) return rc;
+  std::lock_guard<std::mutex> lock(g_dense_mutex);
+  if (g_dense_sms[device] == 0) {
+    int major = 0, count = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+    if (major != 10) return fail("this library targets sm_100a (compute capability 10.x)");
+    cudaError_t e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<64, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<64>::kSmemBytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<128>::kSmemBytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<128>::kSmemBytes);
+    if (e != cudaSuccess) return fail_cuda("dense set-up", e);
+    g_dense_sms[device] = count;
+  }
+  *sms = g_dense_sms[device];
+  return 0;
+}
+
+constexpr uint32_t kDenseMaxSize = 1u << 26;
+
+uint64_t dense_element_bytes(uint32_t dtype) { return dtype == kDenseF32 ? 4 : 2; }
+
+}  // namespace
+
+extern "C" {
+
+int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, float* scale_f32, uint64_t scale_row_stride,
+                                     uint64_t scale_block_stride, const void* x, uint32_t x_dtype, uint64_t x_pitch, uint32_t m,
+                                     uint32_t k, cudaStream_t stream) {
+  if (!codes_fp8 || !scale_f32 || !x) return fail("dense_quantize_rows: null pointer");
+  if (x_dtype > kDenseF32) return fail("dense_quantize_rows: unknown element type");
+  if (m == 0 || k == 0 || m > kDenseMaxSize || k > kDenseMaxSize) return fail("dense_quantize_rows: rows and columns must be 1..2^26");
+  if ((m > 1 && x_pitch < k) || (m > 1 && codes_pitch < k)) return fail("dense_quantize_rows: a row pitch is smaller than the row");
+  if ((uintptr_t)x % dense_element_bytes(x_dtype)) return fail("dense_quantize_rows: input is not aligned to its element");
+  const uint64_t items = (uint64_t)m * ((k + 127) / 128);
+  const uint64_t grid = (items + 15) / 16;
+  if (grid > 0x7fffffffull) return fail("dense_quantize_rows: too many blocks of 128 in one call");
+  netra_dense_quantize_rows_sm100<<<(unsigned)grid, 256, 0, stream>>>(x, x_dtype, x_pitch, (uint8_t*)codes_fp8, codes_pitch, scale_f32,
+                                                                      scale_row_stride, scale_block_stride, m, k);
+  return check_launch("dense_quantize_rows launch");
+}
+
+int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pitch, const void* a_fp8, uint64_t a_pitch,
+                                  const float* a_scale_f32, uint64_t a_scale_row_stride, uint64_t a_scale_block_stride,
+                                  const void* w_fp8, uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch,
+                                  uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols, cudaStream_t stream) {
+  if (!out || !a_fp8 || !a_scale_f32 || !w_fp8 || !w_scale_f32) return fail("dense_fp8_matmul: null pointer");
+  if (out_dtype > kDenseF32) return fail("dense_fp8_matmul: unknown element type");
+  if (transpose_w > 1) return fail("dense_fp8_matmul: transpose_w must be 0 or 1");
+  if (m == 0 || w_rows == 0 || w_cols == 0 || m > kDenseMaxSize || w_rows > kDenseMaxSize || w_cols > kDenseMaxSize)
+    return fail("dense_fp8_matmul: sizes must be 1..2^26");
+  const uint32_t n = transpose_w ? w_cols : w_rows, k = transpose_w ? w_rows : w_cols;
+  if (a_pitch % 16 || w_pitch % 16 || (uintptr_t)a_fp8 % 16 || (uintptr_t)w_fp8 % 16)
+    return fail("dense_fp8_matmul: codes need 16-byte aligned addresses and row pitches");
+  if (a_pitch < k || w_pitch < w_cols || out_pitch < n || w_scale_pitch < (w_cols + 127) / 128)
+    return fail("dense_fp8_matmul: a row pitch is smaller than the row");
+  if ((uintptr_t)out % dense_element_bytes(out_dtype) || (uintptr_t)a_scale_f32 % 4 || (uintptr_t)w_scale_f32 % 4)
+    return fail("dense_fp8_matmul: an address is not aligned to its element");
+  int sms = 0;
+  if (int rc = dense_setup(&sms)) return rc;
+  DnArgs g;
+  g.a_scale = a_scale_f32; g.a_scale_row = a_scale_row_stride; g.a_scale_block = a_scale_block_stride;
+  g.w_scale = w_scale_f32;
+  g.w_scale_col = transpose_w ? 1 : w_scale_pitch;
+  g.w_scale_block = transpose_w ? w_scale_pitch : 1;
+  g.out = out; g.out_pitch = out_pitch; g.out_dtype = out_dtype;
+  g.m = m; g.n = n; g.k_blocks = (k + 127) / 128;
+  const uint64_t m_tiles = (m + 127) / 128;
+  const bool narrow = !transpose_w && m_tiles * ((n + 127) / 128) * 2 <= (uint64_t)sms;
+  const uint32_t bn = narrow ? 64 : 128;
+  g.n_tiles = (n + bn - 1) / bn;
+  const uint64_t tiles = m_tiles * g.n_tiles;
+  uint32_t split = 1;
+  while (split < 8 && tiles * split * 2 <= (uint64_t)sms && g.k_blocks >= split * 4) split *= 2;
+  if (tiles * split > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
+  CUtensorMap tm_a, tm_w;
+  if (int rc = encode_codes(&tm_a, a_fp8, m, k, a_pitch, 128)) return rc;
+  if (int rc = encode_codes(&tm_w, w_fp8, w_rows, w_cols, w_pitch, transpose_w ? 128 : bn)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(tiles * split)); cfg.blockDim = dim3(kDnThreads);
+  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
+  cudaError_t e;
+  if (transpose_w) {
+    cfg.dynamicSmemBytes = DnCfg<128>::kSmemBytes;
+    e = cudaLaunchKernelEx(&cfg, netra_dense_fp8_matmul_sm100<128, true>, tm_a, tm_w, g);
+  } else if (narrow) {
+    cfg.dynamicSmemBytes = DnCfg<64>::kSmemBytes;
+    e = cudaLaunchKernelEx(&cfg, netra_dense_fp8_matmul_sm100<64, false>, tm_a, tm_w, g);
+  } else {
+    cfg.dynamicSmemBytes = DnCfg<128>::kSmemBytes;
+    e = cudaLaunchKernelEx(&cfg, netra_dense_fp8_matmul_sm100<128, false>, tm_a, tm_w, g);
+  }
+  if (e != cudaSuccess) return fail_cuda("dense_fp8_matmul launch", e);
+  return check_launch("dense_fp8_matmul launch");
+}
+
+// codes [m, k rounded up to 16] and, behind them, scales [ceil(k/128)][m]
+uint64_t netra_dense_fp8_linear_workspace_bytes(uint32_t m, uint32_t k) {
+  const uint64_t codes = (uint64_t)m * (((uint64_t)k + 15) / 16 * 16);
+  return codes + (uint64_t)m * ((k + 127ull) / 128) * 4;
+}
+
+int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, uint32_t dtype, uint64_t x_pitch, const void* w_fp8,
+                                  uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch, uint32_t transpose_w, uint32_t m,
+                                  uint32_t w_rows, uint32_t w_cols, void* workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+  const uint32_t k = transpose_w ? w_rows : w_cols;
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < netra_dense_fp8_linear_workspace_bytes(m, k))
+    return fail("dense_fp8_linear: workspace missing, too small or not 16-byte aligned");
+  const uint64_t pitch = ((uint64_t)k + 15) / 16 * 16;
+  uint8_t* codes = (uint8_t*)workspace;
+  float* scale = (float*)(codes + (uint64_t)m * pitch);
+  if (int rc = netra_dense_quantize_rows_launch(codes, pitch, scale, 1, m, x, dtype, x_pitch, m, k, stream)) return rc;
+  return netra_dense_fp8_matmul_launch(out, dtype, out_pitch, codes, pitch, scale, 1, m, w_fp8, w_pitch, w_scale_f32, w_scale_pitch,
+                                       transpose_w, m, w_rows, w_cols, stream);
+}
+
+int netra_dense_status(uint32_t status_out[4]) {
+  if (status_out == nullptr) return fail("dense_status: null pointer");
+  cudaError_t e = cudaMemcpyFromSymbol(status_out, g_dense_status, 16);
+  return e == cudaSuccess ? 0 : fail_cuda("cudaMemcpyFromSymbol(dense status)", e);
+}
+
+}  // extern "C"
