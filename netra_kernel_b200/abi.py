@@ -143,6 +143,17 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def torch_binding():
+    """The torch side of the dense and balance-loss entry points (csrc/torch_binding.cpp).  Raises if it is absent."""
+    load()
+    try:
+        import torch  # noqa: F401  (its libraries have to be in the process first)
+        from .csrc import _netra_torch
+    except ImportError as e:
+        raise RuntimeError(f"csrc/_netra_torch.so cannot be loaded ({e}): build it with `python -m netra_kernel_b200.csrc.build`") from e
+    return _netra_torch
+
+
 class NetraError(RuntimeError):
     pass
 

@@ -27,15 +27,15 @@ def test_cpu_tensors_are_refused():
 def test_weight_checks():
     cpu = torch.device("cpu")
     ok, scale = _fp8(300, 272), torch.ones(3, 3)
-    dense._check_weight(ok, scale, cpu)
-    dense._check_weight(_fp8(300, 288)[:, :260], scale, cpu)                    # padded rows
+    abi.torch_binding().check_weight(ok, scale, cpu)
+    abi.torch_binding().check_weight(_fp8(300, 288)[:, :260], scale, cpu)                    # padded rows
     for weight, s, why in [
         (ok.view(torch.uint8), scale, "float8"), (_fp8(0, 128), torch.ones(0, 1), "float8"),
         (_fp8(300, 260), scale, "16-byte"), (ok.t(), torch.ones(3, 3), "16-byte"), (_fp8(301, 272).view(-1)[16 * 17 - 8:-8].view(300, 272), scale, "16-byte"),
         (ok, torch.ones(3, 2), "weight_scale"), (ok, scale.double(), "weight_scale"), (ok, torch.arange(9.0).view(3, 3).t(), "row-major"),
         (ok, torch.ones(3, 3, requires_grad=True), "frozen")]:
         with pytest.raises(ValueError, match=why):
-            dense._check_weight(weight, s, cpu)
+            abi.torch_binding().check_weight(weight, s, cpu)
 
 
 def test_c_entries_refuse_before_any_launch():
