@@ -19,83 +19,146 @@ netra_expert_counts_sm100(const void* __restrict__ ids, uint32_t wide, uint64_t 
   __shared__ int hist[kBalMaxExperts];
   for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
-  const uint64_t pairs = tokens * slots;
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < pairs; i += (uint64_t)gridDim.x * blockDim.x) {
-    const uint64_t t = i / slots, at = t * id_pitch + (i - t * slots);
-    if (mask != nullptr && mask[t] == 0) continue;
+  const uint32_t pairs = (uint32_t)tokens * slots, step = gridDim.x * 256u;       // the host keeps pairs below 2^31
+#pragma unroll 4
+  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < pairs; i += step) {
+    const uint32_t t = i / slots;
+    const uint64_t at = t * id_pitch + (i - t * slots);
+    const bool live = mask == nullptr || mask[t] != 0;
     const long long id = wide ? reinterpret_cast<const long long*>(ids)[at] : (long long)reinterpret_cast<const int32_t*>(ids)[at];
-    if (id >= 0 && id < (long long)experts) atomicAdd(&hist[id], 1);
+    if (live && id >= 0 && id < (long long)experts) atomicAdd(&hist[id], 1);
   }
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
     if (hist[e] != 0) atomicAdd(&counts[e], hist[e]);
 }
 
-__device__ __forceinline__ float bal_load(const void* z, uint32_t dtype, uint64_t i) { return dense_load(z, dtype, i); }
-
-// share[e] = counts[e] / sum counts (0 where nothing was counted)
-__device__ __forceinline__ void bal_shares(float* share, const int32_t* __restrict__ counts, uint32_t experts) {
-  __shared__ unsigned long long total;
-  if (threadIdx.x == 0) total = 0;
-  __syncthreads();
-  unsigned long long mine = 0;
-  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) mine += (unsigned long long)(long long)counts[e];
-  atomicAdd(&total, mine);
-  __syncthreads();
-  const float inv = total > 0 ? (float)(1.0 / (double)total) : 0.0f;
-  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) share[e] = (float)counts[e] * inv;
-  __syncthreads();
+__device__ __forceinline__ float redux_max_f32(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// one warp, one row: p[i] = softmax of expert lane + 32 i; returns d = sum_e share_e p_e in every lane
-template <int kPer>
-__device__ __forceinline__ float bal_row(float p[kPer], const void* __restrict__ z, uint32_t dtype, uint64_t base, const float* share,
-                                         uint32_t experts, int lane) {
-  float mx = -INFINITY;
+// A lane holds kVec neighbouring experts (16 bytes) of every 32 * kVec.  kAligned: every row allows 16-byte accesses; without
+// it the same lane loads the same experts one by one, so that alignment does not change a sum.
+template <typename T, bool kAligned, int kPer>
+struct BalLane {
+  static constexpr int kVec = 16 / sizeof(T);
+  static_assert(kPer % kVec == 0, "a lane holds whole accesses");
+  __device__ static __forceinline__ uint32_t expert(int i, int lane) { return (uint32_t)((i / kVec) * 32 * kVec + lane * kVec + i % kVec); }
+  __device__ static __forceinline__ void load(float v[kPer], const T* __restrict__ row, uint32_t experts, int lane) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const uint32_t e = lane + 32 * i;
-    p[i] = e < experts ? bal_load(z, dtype, base + e) : -INFINITY;
-    mx = fmaxf(mx, p[i]);
+    for (int i = 0; i < kPer; i += kVec) {
+      const uint32_t e = expert(i, lane);
+      if (kAligned && e < experts) {
+        if constexpr (kVec == 8) {
+          dense_load8(v + i, row + e);
+        } else {
+          const float4 f = *reinterpret_cast<const float4*>(row + e);
+          v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[i + j] = e + j < experts ? dense_load(row, DenseElement<T>::code, e + j) : -INFINITY;
+      }
+    }
   }
-  mx = warp_max(mx);
+  __device__ static __forceinline__ void store(T* __restrict__ row, const float v[kPer], uint32_t experts, int lane) {
+#pragma unroll
+    for (int i = 0; i < kPer; i += kVec) {
+      const uint32_t e = expert(i, lane);
+      if (kAligned && e < experts) {
+        if constexpr (kVec == 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (std::is_same<T, __half>::value) {
+              const __half2 h = __floats2half2_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+              w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+              w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+          *reinterpret_cast<uint4*>(row + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          *reinterpret_cast<float4*>(row + e) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (e + j < experts) dense_store(row, DenseElement<T>::code, e + j, v[i + j]);
+      }
+    }
+  }
+  // the counts of the lane's experts; returns 1 / their sum over the warp (FP32: a common factor, off by a few steps at most)
+  __device__ static __forceinline__ float counts(float c[kPer], const int32_t* __restrict__ all, uint32_t experts, int lane) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = expert(i, lane);
+      c[i] = e < experts ? (float)__ldg(all + e) : 0.0f;
+      sum += c[i];
+    }
+    sum = warp_sum(sum);
+    return sum > 0.0f ? 1.0f / sum : 0.0f;
+  }
+};
+
+// e^x for x <= 0: a hardware base-2 exponential of the rounded product (errors of 2 steps, and |x| 2^-24 from the rounding)
+__device__ __forceinline__ float exp_nonpositive(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
+// v: a row's logits -> its exponentials; returns sum_e c_e p_e in every lane, inv = 1 / sum of the exponentials
+template <int kPer>
+__device__ __forceinline__ float bal_row(float v[kPer], const float c[kPer], float& inv) {
+  float mx = v[0];
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) mx = fmaxf(mx, v[i]);
+  mx = redux_max_f32(mx);
   const float shift = mx == -INFINITY ? 0.0f : mx;
   float sum = 0.0f, dot = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const uint32_t e = lane + 32 * i;
-    p[i] = expf(p[i] - shift);
-    sum += p[i];
-    dot = fmaf(p[i], e < experts ? share[e] : 0.0f, dot);
+    v[i] = exp_nonpositive(v[i] - shift);
+    sum += v[i];
+    dot = fmaf(v[i], c[i], dot);
   }
-  sum = warp_sum(sum);
-  dot = warp_sum(dot);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) p[i] *= inv;
+  for (int d = 16; d > 0; d >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    dot += __shfl_xor_sync(0xffffffffu, dot, d);
+  }
+  inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   return dot * inv;
 }
 
 struct BalPartial { double sum; unsigned long long rows; };
 
-// loss, and scale = E / n; partial: one slot per block, ticket: cleared by the caller
-template <int kPer>
+// A warp per row, a lane holds its experts' counts in registers (no block-wide step before the first row); the rows' d_t are
+// added in FP64: per warp, over the block's warps, over the blocks, always in the same order.  partial: one slot per block;
+// ticket: cleared by the caller.  scale = E / n.
+template <typename T, bool kAligned, int kPer>
 __global__ void __launch_bounds__(kBalThreads)
-netra_balance_loss_sm100(const void* __restrict__ z, uint32_t dtype, uint64_t pitch, const int32_t* __restrict__ counts,
-                         const uint8_t* __restrict__ mask, float* __restrict__ loss, float* __restrict__ scale, BalPartial* __restrict__ partial,
+netra_balance_loss_sm100(const T* __restrict__ z, uint64_t pitch, const int32_t* __restrict__ counts, const uint8_t* __restrict__ mask,
+                         float* __restrict__ loss, float* __restrict__ scale, BalPartial* __restrict__ partial,
                          uint32_t* __restrict__ ticket, uint64_t tokens, uint32_t experts) {
-  __shared__ float share[kBalMaxExperts];
+  using L = BalLane<T, kAligned, kPer>;
   __shared__ double warp_part[kBalThreads / 32];
   __shared__ unsigned long long warp_rows[kBalThreads / 32];
   __shared__ bool last;
-  bal_shares(share, counts, experts);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double sum = 0.0;
   unsigned long long rows = 0;
-  float p[kPer];
+  float c[kPer], v[kPer], inv;
+  const float per_count = L::counts(c, counts, experts, lane);
   for (uint64_t t = (uint64_t)blockIdx.x * (kBalThreads / 32) + warp; t < tokens; t += (uint64_t)gridDim.x * (kBalThreads / 32)) {
     if (mask != nullptr && mask[t] == 0) continue;
-    sum += (double)bal_row<kPer>(p, z, dtype, t * pitch, share, experts, lane);
+    L::load(v, z + t * pitch, experts, lane);
+    sum += (double)(bal_row<kPer>(v, c, inv) * per_count);
     ++rows;
   }
   if (lane == 0) { warp_part[warp] = sum; warp_rows[warp] = rows; }
@@ -108,38 +171,47 @@ netra_balance_loss_sm100(const void* __restrict__ z, uint32_t dtype, uint64_t pi
     last = atomicAdd(ticket, 1u) == gridDim.x - 1;
   }
   __syncthreads();
-  if (!last || warp != 0) return;
+  if (!last) return;
   __threadfence();
   double s = 0.0;
   unsigned long long n = 0;
-  for (uint32_t b = lane; b < gridDim.x; b += 32) { s += __ldcg(&partial[b].sum); n += __ldcg(&partial[b].rows); }
+#pragma unroll 4
+  for (uint32_t b = threadIdx.x; b < gridDim.x; b += kBalThreads) { s += __ldcg(&partial[b].sum); n += __ldcg(&partial[b].rows); }
   for (int d = 16; d > 0; d >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, d); n += __shfl_xor_sync(0xffffffffu, n, d); }
-  if (lane == 0) {
+  if (lane == 0) { warp_part[warp] = s; warp_rows[warp] = n; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    n = 0;
+    for (int w = 0; w < kBalThreads / 32; ++w) { s += warp_part[w]; n += warp_rows[w]; }
     const double per = n > 0 ? (double)experts / (double)n : 0.0;
     *loss = (float)(s * per);
     *scale = (float)per;
   }
 }
 
-template <int kPer>
+template <typename T, bool kAligned, int kPer>
 __global__ void __launch_bounds__(kBalThreads)
-netra_balance_loss_grad_sm100(void* __restrict__ grad, uint64_t grad_pitch, const void* __restrict__ z, uint32_t dtype, uint64_t pitch,
+netra_balance_loss_grad_sm100(T* __restrict__ grad, uint64_t grad_pitch, const T* __restrict__ z, uint64_t pitch,
                               const int32_t* __restrict__ counts, const uint8_t* __restrict__ mask, const float* __restrict__ scale,
                               const float* __restrict__ upstream, uint64_t tokens, uint32_t experts) {
-  __shared__ float share[kBalMaxExperts];
-  bal_shares(share, counts, experts);
+  using L = BalLane<T, kAligned, kPer>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float k = scale[0] * upstream[0];
-  float p[kPer];
+  float c[kPer], v[kPer], inv;
+  const float per_count = L::counts(c, counts, experts, lane);
+  const float k = *scale * *upstream;
   for (uint64_t t = (uint64_t)blockIdx.x * (kBalThreads / 32) + warp; t < tokens; t += (uint64_t)gridDim.x * (kBalThreads / 32)) {
-    const bool live = mask == nullptr || mask[t] != 0;
-    float d = 0.0f;
-    if (live) d = bal_row<kPer>(p, z, dtype, t * pitch, share, experts, lane);
+    if (mask == nullptr || mask[t] != 0) {
+      L::load(v, z + t * pitch, experts, lane);
+      const float d = bal_row<kPer>(v, c, inv);
+      // p_te (f_e - d_t) = p_te (c_e - sum_j c_j p_tj) / total: whole counts are subtracted, the quotient comes last
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t e = lane + 32 * i;
-      if (e < experts) dense_store(grad, dtype, t * grad_pitch + e, live ? p[i] * (share[e] - d) * k : 0.0f);
+      for (int i = 0; i < kPer; ++i) v[i] = v[i] * inv * ((c[i] - d) * per_count) * k;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = 0.0f;
     }
+    L::store(grad + t * grad_pitch, v, experts, lane);
   }
 }
 
@@ -147,7 +219,7 @@ netra_balance_loss_grad_sm100(void* __restrict__ grad, uint64_t grad_pitch, cons
 
 namespace {
 
-constexpr uint32_t kBalMaxBlocks = 1184;      // eight blocks per SM of a 148-SM device
+constexpr uint32_t kBalMaxBlocks = 592;       // four blocks per SM of a 148-SM device: more warps only repeat the look at the counts
 
 int balance_check(const char* what, const void* z, uint32_t dtype, uint64_t pitch, const void* counts, uint64_t tokens, uint32_t experts) {
   static thread_local char text[128];
@@ -166,6 +238,27 @@ uint32_t balance_blocks(uint64_t tokens) {
   return (uint32_t)(b < kBalMaxBlocks ? b : kBalMaxBlocks);
 }
 
+// Calls f(element, 16-byte accesses?, experts per lane) with the smallest register file that holds a row.
+template <typename F>
+void balance_shape(uint32_t dtype, bool aligned, uint32_t experts, F&& f) {
+  auto sized = [&](auto element, auto access) {
+    if constexpr (sizeof(element) == 4) {
+      if (experts <= 128) { f(element, access, std::integral_constant<int, 4>{}); return; }
+    }
+    if (experts <= 256) f(element, access, std::integral_constant<int, 8>{});
+    else if (experts <= 512) f(element, access, std::integral_constant<int, 16>{});
+    else f(element, access, std::integral_constant<int, 32>{});
+  };
+  auto typed = [&](auto element) { if (aligned) sized(element, std::true_type{}); else sized(element, std::false_type{}); };
+  if (dtype == kDenseF32) typed(0.0f);
+  else if (dtype == kDenseF16) typed(__half{});
+  else typed(__nv_bfloat16{});
+}
+bool balance_aligned(const void* p, uint64_t pitch, uint32_t dtype, uint32_t experts) {
+  const uint64_t size = dense_element_bytes(dtype);
+  return (uintptr_t)p % 16 == 0 && pitch * size % 16 == 0 && experts * size % 16 == 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -182,7 +275,7 @@ int netra_expert_counts_launch(int32_t* counts_i32, const void* ids, uint32_t id
   if (e != cudaSuccess) return fail_cuda("expert_counts memset", e);
   const uint64_t pairs = tokens * slots;
   if (pairs == 0) return 0;
-  const uint64_t blocks = (pairs + 1023) / 1024;
+  const uint64_t blocks = (pairs + 511) / 512;
   netra_expert_counts_sm100<<<(unsigned)(blocks < 296 ? blocks : 296), 256, 0, stream>>>(ids, id_bytes == 8, id_pitch, token_mask, counts_i32,
                                                                                         tokens, slots, experts);
   return check_launch("expert_counts launch");
@@ -201,13 +294,11 @@ int netra_balance_loss_launch(float* loss_f32, float* scale_f32, const void* log
   cudaError_t e = cudaMemsetAsync(ticket, 0, sizeof(uint32_t), stream);
   if (e != cudaSuccess) return fail_cuda("balance_loss memset", e);
   const uint32_t grid = balance_blocks(tokens);
-  auto launch = [&](auto per) {
-    netra_balance_loss_sm100<decltype(per)::value><<<grid, kBalThreads, 0, stream>>>(logits, dtype, pitch, counts_i32, token_mask, loss_f32, scale_f32,
-                                                                                    partial, ticket, tokens, experts);
-  };
-  if (experts <= 64) launch(std::integral_constant<int, 2>{});
-  else if (experts <= 256) launch(std::integral_constant<int, 8>{});
-  else launch(std::integral_constant<int, 32>{});
+  balance_shape(dtype, balance_aligned(logits, pitch, dtype, experts), experts, [&](auto element, auto access, auto per) {
+    using T = decltype(element);
+    netra_balance_loss_sm100<T, decltype(access)::value, decltype(per)::value><<<grid, kBalThreads, 0, stream>>>(
+        (const T*)logits, pitch, counts_i32, token_mask, loss_f32, scale_f32, partial, ticket, tokens, experts);
+  });
   return check_launch("balance_loss launch");
 }
 
@@ -219,13 +310,12 @@ int netra_balance_loss_grad_launch(void* grad, uint64_t grad_pitch, const void* 
   if (tokens > 1 && grad_pitch < experts) return fail("balance_loss_grad: a row pitch is smaller than the row");
   if ((uintptr_t)grad % dense_element_bytes(dtype)) return fail("balance_loss_grad: the gradient is not aligned to its element");
   const uint32_t grid = balance_blocks(tokens);
-  auto launch = [&](auto per) {
-    netra_balance_loss_grad_sm100<decltype(per)::value><<<grid, kBalThreads, 0, stream>>>(grad, grad_pitch, logits, dtype, pitch, counts_i32, token_mask,
-                                                                                         scale_f32, upstream_f32, tokens, experts);
-  };
-  if (experts <= 64) launch(std::integral_constant<int, 2>{});
-  else if (experts <= 256) launch(std::integral_constant<int, 8>{});
-  else launch(std::integral_constant<int, 32>{});
+  const bool aligned = balance_aligned(logits, pitch, dtype, experts) && balance_aligned(grad, grad_pitch, dtype, experts);
+  balance_shape(dtype, aligned, experts, [&](auto element, auto access, auto per) {
+    using T = decltype(element);
+    netra_balance_loss_grad_sm100<T, decltype(access)::value, decltype(per)::value><<<grid, kBalThreads, 0, stream>>>(
+        (T*)grad, grad_pitch, (const T*)logits, pitch, counts_i32, token_mask, scale_f32, upstream_f32, tokens, experts);
+  });
   return check_launch("balance_loss_grad launch");
 }
 

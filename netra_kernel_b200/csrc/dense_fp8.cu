@@ -28,38 +28,93 @@ __device__ __forceinline__ void dense_store(void* p, uint32_t dtype, size_t i, f
 }
 
 // ------------------------------------------------------------------------------------------
-// Row quantiser.  Sixteen lanes own one block of 128 columns, eight neighbouring columns each.
-// Scales go to scale[m * scale_row + b * scale_block].
+// Row quantiser.  Sixteen lanes own one block of 128 columns of kRows neighbouring rows, eight neighbouring columns each: a
+// BF16 lane loads 16 bytes and stores 8 codes.  HBM bound; the four rows of the large form keep four loads in flight per
+// lane, and let one lane store the block's four scales side by side (scales are stored block by block).
+// Scales go to scale[m * scale_row + b * scale_block].  kVector: eight columns are one aligned access and lie wholly inside
+// or outside the row.
 // ------------------------------------------------------------------------------------------
-extern "C" __global__ void __launch_bounds__(256)
-netra_dense_quantize_rows_sm100(const void* __restrict__ x, uint32_t dtype, uint64_t x_pitch, uint8_t* __restrict__ codes,
-                                uint64_t codes_pitch, float* __restrict__ scale, uint64_t scale_row, uint64_t scale_block,
-                                uint32_t m, uint32_t k) {
-  const uint32_t blocks = (k + kBlock - 1) / kBlock;
-  const uint64_t total = (uint64_t)m * blocks;
-  const int sub = threadIdx.x & 15;
-  const uint64_t item = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
-  const bool live = item < total;
-  const uint64_t row = live ? item / blocks : 0;
-  const uint32_t b = live ? (uint32_t)(item - row * blocks) : 0;
-  float v[8];
-  float amax = amax_floor();
+template <typename T> struct DenseElement;
+template <> struct DenseElement<__nv_bfloat16> { static constexpr uint32_t code = kDenseBf16; };
+template <> struct DenseElement<__half> { static constexpr uint32_t code = kDenseF16; };
+template <> struct DenseElement<float> { static constexpr uint32_t code = kDenseF32; };
+
+// eight elements at p (16-byte aligned; 32 bytes of FP32)
+template <typename T>
+__device__ __forceinline__ void dense_load8(float v[8], const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t col = b * kBlock + sub * 8 + j;
-    v[j] = live && col < k ? dense_load(x, dtype, row * x_pitch + col) : 0.0f;
-    amax = fmaxf(amax, fabsf(v[j]));
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[2 * j] = f.x; v[2 * j + 1] = f.y;
+      } else {
+        v[2 * j] = bf16_bits_to_f32(w[j] & 0xffffu); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  }
+}
+
+template <typename T, bool kVector, int kRows>
+__global__ void __launch_bounds__(256)
+netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8_t* __restrict__ codes, uint64_t codes_pitch,
+                                float* __restrict__ scale, uint64_t scale_row, uint64_t scale_block, uint32_t m, uint32_t k) {
+  const uint32_t blocks = (k + kBlock - 1) / kBlock;
+  const uint32_t item = (blockIdx.x * 256u + threadIdx.x) >> 4;
+  const uint32_t group = item / blocks, b = item - group * blocks;
+  const uint64_t row0 = (uint64_t)group * kRows;
+  const uint32_t col = b * kBlock + (threadIdx.x & 15) * 8;
+  float v[kRows][8], s[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const bool live = row0 + r < m;
+    const T* src = x + (row0 + r) * x_pitch + col;
+    if (kVector) {
+      if (live && col < k) {
+        dense_load8(v[r], src);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[r][j] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[r][j] = live && col + j < k ? dense_load(src, DenseElement<T>::code, j) : 0.0f;
+    }
   }
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-  if (!live) return;
-  const float s = amax * inv448();
-  const float inv = 1.0f / s;
-  if (sub == 0) scale[row * scale_row + b * scale_block] = s;
+  for (int r = 0; r < kRows; ++r) {
+    float amax = amax_floor();
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t col = b * kBlock + sub * 8 + j;
-    if (col < k) codes[row * codes_pitch + col] = f32_to_e4m3(v[j] * inv);
+    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[r][j]));
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    s[r] = amax * inv448();
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (row0 + r >= m) break;
+    const float inv = 1.0f / s[r];
+    uint8_t* dst = codes + (row0 + r) * codes_pitch + col;
+    const uint32_t lo = f32x4_to_e4m3x4(v[r][0] * inv, v[r][1] * inv, v[r][2] * inv, v[r][3] * inv);
+    const uint32_t hi = f32x4_to_e4m3x4(v[r][4] * inv, v[r][5] * inv, v[r][6] * inv, v[r][7] * inv);
+    if (kVector) {
+      if (col < k) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < k) dst[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    }
+  }
+  if ((threadIdx.x & 15) == 0) {
+    float* dst = scale + row0 * scale_row + b * scale_block;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (row0 + r < m) dst[r * scale_row] = s[r];
   }
 }
 
@@ -322,11 +377,26 @@ int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, floa
   if (m == 0 || k == 0 || m > kDenseMaxSize || k > kDenseMaxSize) return fail("dense_quantize_rows: rows and columns must be 1..2^26");
   if ((m > 1 && x_pitch < k) || (m > 1 && codes_pitch < k)) return fail("dense_quantize_rows: a row pitch is smaller than the row");
   if ((uintptr_t)x % dense_element_bytes(x_dtype)) return fail("dense_quantize_rows: input is not aligned to its element");
-  const uint64_t items = (uint64_t)m * ((k + 127) / 128);
-  const uint64_t grid = (items + 15) / 16;
-  if (grid > 0x7fffffffull) return fail("dense_quantize_rows: too many blocks of 128 in one call");
-  netra_dense_quantize_rows_sm100<<<(unsigned)grid, 256, 0, stream>>>(x, x_dtype, x_pitch, (uint8_t*)codes_fp8, codes_pitch, scale_f32,
-                                                                      scale_row_stride, scale_block_stride, m, k);
+  const uint64_t blocks = (k + 127) / 128;
+  // four rows per lane once that still leaves every SM a few thousand lanes; below, one row each for the shortest chain
+  const bool deep = (uint64_t)m * blocks >= 32768;
+  const uint64_t grid = ((deep ? (m + 3) / 4 : m) * blocks + 15) / 16;
+  if (grid > 0x0fffffffull) return fail("dense_quantize_rows: too many blocks of 128 in one call");
+  const bool vector = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (x_pitch * dense_element_bytes(x_dtype)) % 16 == 0 &&
+                      (uintptr_t)codes_fp8 % 8 == 0 && codes_pitch % 8 == 0;
+  auto launch = [&](auto element, auto vec, auto rows) {
+    using T = decltype(element);
+    netra_dense_quantize_rows_sm100<T, decltype(vec)::value, decltype(rows)::value><<<(unsigned)grid, 256, 0, stream>>>(
+        (const T*)x, x_pitch, (uint8_t*)codes_fp8, codes_pitch, scale_f32, scale_row_stride, scale_block_stride, m, k);
+  };
+  auto shape = [&](auto element) {
+    if (!vector) { if (deep) launch(element, std::false_type{}, std::integral_constant<int, 4>{}); else launch(element, std::false_type{}, std::integral_constant<int, 1>{}); }
+    else if (deep) launch(element, std::true_type{}, std::integral_constant<int, 4>{});
+    else launch(element, std::true_type{}, std::integral_constant<int, 1>{});
+  };
+  if (x_dtype == kDenseBf16) shape(__nv_bfloat16{});
+  else if (x_dtype == kDenseF16) shape(__half{});
+  else shape(0.0f);
   return check_launch("dense_quantize_rows launch");
 }
 
