@@ -316,7 +316,11 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
 
 }  // namespace netra
 
+#include "dense_pair.cu"
+
 namespace {
+
+uint64_t dense_element_bytes(uint32_t dtype) { return dtype == kDenseF32 ? 4 : 2; }
 
 // Byte tensor of `rows` rows of `cols` codes, `pitch` bytes apart; box 128 bytes x box_rows, 128-byte swizzle.
 int encode_codes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
@@ -336,10 +340,28 @@ int encode_codes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t col
   return 0;
 }
 
+// Output matrix of 2- or 4-byte elements; box 128 bytes x 32 rows, 128-byte swizzle.
+int encode_output(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t element_bytes) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return fail("cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch * element_bytes};
+  cuuint32_t box[2] = {128 / element_bytes, 32};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, element_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_error, sizeof g_error, "cuTensorMapEncodeTiled (output) failed with CUresult %d", (int)r);
+    return -1;
+  }
+  return 0;
+}
+
 std::mutex g_dense_mutex;
+bool g_dense_pair_ok[kMaxDevices] = {};   // the pair kernels were built with the register allocation they assume
 int g_dense_sms[kMaxDevices] = {};      // SM count once the kernels of a device are set up
 
-int dense_setup(int* sms) {
+int dense_setup(int* sms, bool* pair_ok) {
   int device = 0;
   if (int rc = current_device_index(&device)) return rc;
   std::lock_guard<std::mutex> lock(g_dense_mutex);
@@ -354,16 +376,23 @@ int dense_setup(int* sms) {
       e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<128>::kSmemBytes);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<128>::kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(netra_dense_fp8_pair_sm100<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(netra_dense_fp8_pair_sm100<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes);
+    // the register re-balancing inside the pair kernels is only deadlock-free for the launch allocation it was written for
+    cudaFuncAttributes plain, transposed;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&plain, netra_dense_fp8_pair_sm100<false>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&transposed, netra_dense_fp8_pair_sm100<true>);
     if (e != cudaSuccess) return fail_cuda("dense set-up", e);
+    g_dense_pair_ok[device] = plain.numRegs == kPairRegsLaunch && transposed.numRegs == kPairRegsLaunch;
     g_dense_sms[device] = count;
   }
   *sms = g_dense_sms[device];
+  *pair_ok = g_dense_pair_ok[device];
   return 0;
 }
 
 constexpr uint32_t kDenseMaxSize = 1u << 26;
 
-uint64_t dense_element_bytes(uint32_t dtype) { return dtype == kDenseF32 ? 4 : 2; }
 
 }  // namespace
 
@@ -417,7 +446,30 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   if ((uintptr_t)out % dense_element_bytes(out_dtype) || (uintptr_t)a_scale_f32 % 4 || (uintptr_t)w_scale_f32 % 4)
     return fail("dense_fp8_matmul: an address is not aligned to its element");
   int sms = 0;
-  if (int rc = dense_setup(&sms)) return rc;
+  bool pair_ok = false;
+  if (int rc = dense_setup(&sms, &pair_ok)) return rc;
+  CUtensorMap tm_a, tm_w;
+  if (int rc = encode_codes(&tm_a, a_fp8, m, k, a_pitch, 128)) return rc;
+  const uint64_t m256 = (m + 255) / 256, n256 = (n + 255) / 256;
+  if (pair_ok && m256 * n256 * 2 > (uint64_t)sms * 3 / 4) {
+    if (m256 * n256 > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
+    PairArgs p;
+    p.a_scale = a_scale_f32; p.a_scale_row = a_scale_row_stride; p.a_scale_block = a_scale_block_stride;
+    p.w_scale = w_scale_f32;
+    p.w_scale_col = transpose_w ? 1 : w_scale_pitch; p.w_scale_block = transpose_w ? w_scale_pitch : 1;
+    p.out = out; p.out_pitch = out_pitch; p.out_dtype = out_dtype;
+    p.m = m; p.n = n; p.k_blocks = (k + 127) / 128; p.m_tiles = (uint32_t)m256; p.n_tiles = (uint32_t)n256;
+    const uint32_t size = (uint32_t)dense_element_bytes(out_dtype);
+    p.tma_store = (uintptr_t)out % 16 == 0 && out_pitch * size % 16 == 0;
+    CUtensorMap tm_out = {};
+    if (int rc = encode_codes(&tm_w, w_fp8, w_rows, w_cols, w_pitch, 128)) return rc;
+    if (p.tma_store)
+      if (int rc = encode_output(&tm_out, out, m, n, out_pitch, size)) return rc;
+    const uint64_t pairs = m256 * n256 < (uint64_t)(sms / 2) ? m256 * n256 : (uint64_t)(sms / 2);
+    if (transpose_w) netra_dense_fp8_pair_sm100<true><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
+    else netra_dense_fp8_pair_sm100<false><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
+    return check_launch("dense_fp8_matmul launch");
+  }
   DnArgs g;
   g.a_scale = a_scale_f32; g.a_scale_row = a_scale_row_stride; g.a_scale_block = a_scale_block_stride;
   g.w_scale = w_scale_f32;
@@ -433,8 +485,6 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   uint32_t split = 1;
   while (split < 8 && tiles * split * 2 <= (uint64_t)sms && g.k_blocks >= split * 4) split *= 2;
   if (tiles * split > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
-  CUtensorMap tm_a, tm_w;
-  if (int rc = encode_codes(&tm_a, a_fp8, m, k, a_pitch, 128)) return rc;
   if (int rc = encode_codes(&tm_w, w_fp8, w_rows, w_cols, w_pitch, transpose_w ? 128 : bn)) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

@@ -1,0 +1,273 @@
+// The dense block-scaled product for many rows: a pair of CTAs (cta_group::2) owns 256 rows x 256 columns of the output.
+//
+// Every K-block of 128 leaves 256 x 256 raw sums in TMEM which the CUDA cores scale by sa[row] * sw[tile] and add up in
+// registers, so three things have to overlap: the tensor core (512 cycles a K-block), the operands (32 KB per CTA and
+// K-block: a pair fetches its weight tile once, half each; one CTA alone would need 48 KB, more than the L2 delivers in that
+// time) and the promotion (128 KB read out of TMEM and 32,768 multiply-adds per CTA).  Sixteen promotion warps, four per
+// scheduler, hide the latencies of that chain that eight cannot; a thread keeps 64 columns of its row.
+//   warp 0: TMA producer (each CTA its own 128 rows and its own 128 weight rows; both report to the leader's barrier)
+//   warp 1: MMA issuer (leader CTA only; owns TMEM), warps 2-3: idle, warps 4..19: promotion and store
+// The grid is persistent; the accumulators are double-buffered in TMEM, so the next item's first two K-blocks run while an
+// item is being stored.  Every wait is bounded; on expiry the CTA records a code and drains.
+namespace netra {
+
+constexpr int kPairThreads = 640;
+// setmaxnreg: the four promotion warpgroups may ask for what the first one gives back, 128 * (96 - 32) = 4 * 128 * (112 - 96)
+constexpr int kPairRegsLaunch = 96, kPairRegsLow = 32, kPairRegsHigh = 112;
+static_assert(128 * kPairRegsLow + 512 * kPairRegsHigh <= kPairThreads * kPairRegsLaunch, "the promotion warps would wait forever for registers");
+
+struct PairCfg {
+  static constexpr int kStages = 5;
+  static constexpr int kStageBytes = 2 * 128 * kBlock;            // 128 rows, 128 weight rows (or columns)
+  static constexpr int kStagingBytes = 16 * 4096;                 // per promotion warp: 32 rows of 128 bytes, swizzled
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 256;
+  static_assert(kSmemBytes <= 232448, "exceeds the shared memory of one SM");
+};
+
+struct PairArgs {
+  const float* a_scale;
+  uint64_t a_scale_row, a_scale_block;
+  const float* w_scale;
+  uint64_t w_scale_col, w_scale_block;
+  void* out;
+  uint64_t out_pitch;
+  uint32_t out_dtype;
+  uint32_t tma_store;                     // rows of the output start on 16-byte boundaries
+  uint32_t m, n, k_blocks;
+  uint32_t m_tiles, n_tiles;              // of 256
+};
+
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// Arrival on a barrier of either CTA of the pair.  It hands over TMEM columns, whose reads tcgen05.wait::ld has completed and
+// tcgen05.fence orders; no other memory is handed over.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// a load into this CTA's shared memory that reports its bytes to a barrier of the pair's leader
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;"
+      ::"r"(dst), "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// one arrival on this barrier of both CTAs once the MMAs issued so far are done
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)map), "r"(src), "r"(x), "r"(y) : "memory");
+}
+// (a.x, a.y) * (s, s) + (c.x, c.y), each component rounded once
+__device__ __forceinline__ float2 fma2(float2 a, float2 s, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&s)), "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+
+// Item i -> tile: columns of eight row tiles, so that the items in flight share few weight and activation tiles in the L2.
+__device__ __forceinline__ void pair_item(uint32_t i, uint32_t m_tiles, uint32_t n_tiles, uint32_t& mt, uint32_t& nt) {
+  const uint32_t band = i / (8 * n_tiles), first = band * 8, rows = min(8u, m_tiles - first), j = i - band * 8 * n_tiles;
+  mt = first + j % rows;
+  nt = j / rows;
+}
+
+template <bool kTransposed>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                           const __grid_constant__ CUtensorMap tm_out, const PairArgs g) {
+  using C = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* staging = smem + C::kStages * C::kStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes);
+  uint64_t* empty_bar = full_bar + C::kStages;
+  uint64_t* tfull_bar = empty_bar + C::kStages;       // [2]
+  uint64_t* tempty_bar = tfull_bar + 2;               // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t items = g.m_tiles * g.n_tiles, pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 32); }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();                                  // the peer's barriers exist before anything reports to them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairRegsLow));
+    if (warp == 0 && lane == 0) {
+      const uint64_t pol = policy_evict_last();
+      uint32_t it = 0;
+      bool ok = true;
+      for (uint32_t item = pair; ok && item < items; item += pairs) {
+        uint32_t mt, nt;
+        pair_item(item, g.m_tiles, g.n_tiles, mt, nt);
+        const int row = (int)(mt * 256 + rank * 128), col = (int)(nt * 256 + rank * 128);
+        for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
+          const uint32_t s = it % C::kStages;
+          if (!mbar_wait(smem_u32(&empty_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
+            g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; ok = false; break;
+          }
+          if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * C::kStageBytes);
+          const uint32_t bar = map_to_rank(smem_u32(&full_bar[s]), 0), dst = smem_u32(smem + s * C::kStageBytes);
+          tma_load_2d_pair(dst, &tm_a, bar, (int)(kb * kBlock), row, pol);
+          if (kTransposed) tma_load_2d_pair(dst + 128 * kBlock, &tm_w, bar, col, (int)(kb * kBlock), pol);
+          else tma_load_2d_pair(dst + 128 * kBlock, &tm_w, bar, (int)(kb * kBlock), col, pol);
+        }
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      const uint32_t idesc = (1u << 4) | (kTransposed ? 1u << 16 : 0u) | ((256u >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+      uint32_t it = 0;
+      bool ok = true;
+      for (uint32_t item = pair; ok && item < items; item += pairs) {
+        for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
+          const uint32_t s = it % C::kStages, a = it & 1;
+          if (!mbar_wait(smem_u32(&tempty_bar[a]), ((it >> 1) & 1) ^ 1, abort_flag) ||
+              !mbar_wait(smem_u32(&full_bar[s]), (it / C::kStages) & 1, abort_flag)) {
+            g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; ok = false; break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
+          const uint64_t adesc = make_smem_desc(sa);
+          const uint64_t bdesc = kTransposed ? make_smem_desc_mn(sa + 128 * kBlock) : make_smem_desc(sa + 128 * kBlock);
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k)
+            umma_f8_pair(tmem_base + a * 256, adesc + 2 * k, bdesc + (kTransposed ? 256 : 2) * k, idesc, k > 0);
+          umma_commit_pair(smem_u32(&empty_bar[s]));
+          umma_commit_pair(smem_u32(&tfull_bar[a]));
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairRegsHigh));
+    const int wg = (warp - 4) >> 2, quad = warp & 3;            // 64 columns and 32 rows of this warp
+    uint8_t* tile = staging + (warp - 4) * 4096;
+    const uint32_t tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(wg * 64);
+    uint32_t it = 0;
+    bool ok = true;
+    for (uint32_t item = pair; item < items; item += pairs) {
+      uint32_t mt, nt;
+      pair_item(item, g.m_tiles, g.n_tiles, mt, nt);
+      const uint32_t row0 = mt * 256 + rank * 128 + quad * 32, col0 = nt * 256 + wg * 64;
+      const float* sa_ptr = g.a_scale + (uint64_t)min(row0 + lane, g.m - 1) * g.a_scale_row;
+      const float* sw_ptr = g.w_scale + (uint64_t)(min(col0, g.n - 1) / kBlock) * g.w_scale_col;
+      float2 acc[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = make_float2(0.0f, 0.0f);
+      // the scales of the next two K-blocks are on their way while one is being promoted
+      float sa0 = __ldg(sa_ptr), sw0 = __ldg(sw_ptr);
+      const uint32_t second = min(1u, g.k_blocks - 1);
+      float sa1 = __ldg(sa_ptr + second * g.a_scale_block), sw1 = __ldg(sw_ptr + second * g.w_scale_block);
+      for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
+        const uint32_t a = it & 1;
+        const float s = __fmul_rn(sa0, sw0);
+        const uint32_t ahead = min(kb + 2, g.k_blocks - 1);
+        sa0 = sa1; sw0 = sw1;
+        sa1 = __ldg(sa_ptr + ahead * g.a_scale_block); sw1 = __ldg(sw_ptr + ahead * g.w_scale_block);
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (it >> 1) & 1, abort_flag))) {
+          g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; ok = false;
+        }
+        if (!ok) continue;
+        tc_fence_after();
+        const float2 s2 = make_float2(s, s);
+        uint32_t v[32];
+        tmem_ld32_nowait(tbase + a * 256, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 16; ++c) acc[c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), s2, acc[c]);
+        tmem_ld32_nowait(tbase + a * 256 + 32, v);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_pair(map_to_rank(smem_u32(&tempty_bar[a]), 0));
+#pragma unroll
+        for (int c = 0; c < 16; ++c) acc[16 + c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), s2, acc[16 + c]);
+      }
+      // ---- store: 128 bytes per row at a time through this warp's own staging rows (chunk j of row r at j ^ (r & 7), the
+      // 128-byte swizzle of the copy engine), 64 columns of a 16-bit type or 32 of FP32
+      const bool wide = g.out_dtype == kDenseF32;
+      const uint32_t per_pass = wide ? 32 : 64;
+#pragma unroll
+      for (int pass = 0; pass < 2; ++pass) {
+        if (pass == 1 && !wide) break;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the last copy has left the rows
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t p[4];
+          if (wide) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) { const float2 f = acc[pass * 16 + 2 * j + q]; p[2 * q] = __float_as_uint(f.x); p[2 * q + 1] = __float_as_uint(f.y); }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float2 f = acc[4 * j + q];
+              if (g.out_dtype == kDenseF16) { const __half2 h = __floats2half2_rn(f.x, f.y); p[q] = *reinterpret_cast<const uint32_t*>(&h); }
+              else { const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y); p[q] = *reinterpret_cast<const uint32_t*>(&h); }
+            }
+          }
+          *reinterpret_cast<uint4*>(tile + lane * 128 + 16 * (j ^ (lane & 7))) = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+        const uint32_t col = col0 + pass * 32;
+        if (g.tma_store) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < g.m && col < g.n) tma_store_2d(&tm_out, smem_u32(tile), (int)col, (int)row0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          for (uint32_t r = 0; r < 32 && row0 + r < g.m; ++r)
+            for (uint32_t c = lane; c < per_pass && col + c < g.n; c += 32) {
+              const uint32_t byte = c * (wide ? 4 : 2);
+              const uint8_t* src = tile + r * 128 + 16 * ((byte >> 4) ^ (r & 7)) + (byte & 15);
+              const uint64_t at = (uint64_t)(row0 + r) * g.out_pitch + col + c;
+              if (wide) reinterpret_cast<uint32_t*>(g.out)[at] = *reinterpret_cast<const uint32_t*>(src);
+              else reinterpret_cast<uint16_t*>(g.out)[at] = *reinterpret_cast<const uint16_t*>(src);
+            }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) __nanosleep(200000);          // copies in flight land before the CTA exits
+  cluster_barrier();                                  // nothing reports to this CTA any more
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+}  // namespace netra

@@ -120,6 +120,29 @@ def test_linear_against_64_bits(m, n, k):
     dense.check_status()
 
 
+# outputs of many tiles: whole and ragged in every direction, one K-block and several, each element type and pitch
+LARGE = [(2500, 2312, 400, torch.bfloat16), (700, 8200, 144, torch.float16), (4097, 1043, 272, torch.float32), (2305, 2305, 16, torch.bfloat16),
+         (2048, 2560, 1024, torch.float32), (9000, 520, 528, torch.float16)]
+
+
+@pytest.mark.parametrize("m,n,k,dtype", LARGE)
+def test_large_products_against_64_bits(m, n, k, dtype):
+    g = torch.Generator().manual_seed(m + n)
+    x = (torch.randn(m, k, generator=g) * torch.exp(torch.randn(m, 1, generator=g))).to(dtype)
+    w, ws = make_weight(n, k, n + k)
+    frame = torch.full((m + 1, n + 3), 7.0, device="cuda", dtype=dtype)
+    check_product(dense.fp8_linear(x.cuda(), w, ws), *quantize_definition(x), w, ws)
+    codes, scale = dense.quantize_rows(x.cuda())
+    y = dense.block_scaled_matmul(codes, scale, w, ws, out=frame[:-1, 2:-1])
+    check_product(y, *quantize_definition(x), w, ws)
+    assert bool((frame[-1] == 7.0).all()) and bool((frame[:, :2] == 7.0).all()) and bool((frame[:, -1] == 7.0).all())
+    # the same sizes with the weight as stored: [m, k] codes times [k, n]
+    w, ws = make_weight(k, n, n)
+    y = dense.block_scaled_matmul(codes, scale, w, ws, transpose_weight=True, out_dtype=dtype)
+    check_product(y, *quantize_definition(x), w, ws, True)
+    dense.check_status()
+
+
 @pytest.mark.parametrize("m,n,k", SIZES)
 def test_transposed_product_against_64_bits(m, n, k):
     """The gradient form: [m, n] codes times the weight [n, k] as stored."""
