@@ -6,7 +6,9 @@
 // time) and the promotion (128 KB read out of TMEM and 32,768 multiply-adds per CTA).  Sixteen promotion warps, four per
 // scheduler, hide the latencies of that chain that eight cannot; a thread keeps 64 columns of its row.
 //   warp 0: TMA producer (each CTA its own 128 rows and its own 128 weight rows; both report to the leader's barrier)
-//   warp 1: MMA issuer (leader CTA only; owns TMEM), warps 2-3: idle, warps 4..19: promotion and store
+//   warp 1: MMA issuer (leader CTA only; owns TMEM), warp 2: scales, warp 3: idle, warps 4..19: promotion and store
+// The scales go through shared memory, four K-blocks ahead: loaded by the promotion warps themselves, one K-block ahead, they
+// were what the loop waited for (785 ns a K-block against 600 with the loads dropped).
 // The grid is persistent; the accumulators are double-buffered in TMEM, so the next item's first two K-blocks run while an
 // item is being stored.  Every wait is bounded; on expiry the CTA records a code and drains.
 namespace netra {
@@ -17,10 +19,12 @@ constexpr int kPairRegsLaunch = 96, kPairRegsLow = 32, kPairRegsHigh = 112;
 static_assert(128 * kPairRegsLow + 512 * kPairRegsHigh <= kPairThreads * kPairRegsLaunch, "the promotion warps would wait forever for registers");
 
 struct PairCfg {
-  static constexpr int kStages = 5;
+  static constexpr int kStages = 4;
   static constexpr int kStageBytes = 2 * 128 * kBlock;            // 128 rows, 128 weight rows (or columns)
   static constexpr int kStagingBytes = 16 * 4096;                 // per promotion warp: 32 rows of 128 bytes, swizzled
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 256;
+  static constexpr int kScaleSlots = 8;                           // K-blocks whose scales are in shared memory or on their way
+  static constexpr int kScaleSlotFloats = 128 + 4;                // 128 rows, two weight tiles
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kScaleSlots * kScaleSlotFloats * 4 + 256;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of one SM");
 };
 
@@ -45,7 +49,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 // Arrival on a barrier of either CTA of the pair.  It hands over TMEM columns, whose reads tcgen05.wait::ld has completed and
 // tcgen05.fence orders; no other memory is handed over.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_f32(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 // a load into this CTA's shared memory that reports its bytes to a barrier of the pair's leader
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, uint64_t policy) {
@@ -91,7 +98,8 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = smem + C::kStages * C::kStageBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes);
+  float* scales = reinterpret_cast<float*>(staging + C::kStagingBytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kScaleSlots * C::kScaleSlotFloats);
   uint64_t* empty_bar = full_bar + C::kStages;
   uint64_t* tfull_bar = empty_bar + C::kStages;       // [2]
   uint64_t* tempty_bar = tfull_bar + 2;               // [2]
@@ -104,7 +112,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 32); }
+    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 2); mbar_init(smem_u32(&tempty_bar[a]), 32); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -163,6 +171,43 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
           umma_commit_pair(smem_u32(&tfull_bar[a]));
         }
       }
+    } else if (warp == 2) {
+      // An accumulator stage counts as full when its MMAs are done and its K-block's scales are in their slot.  Once K-block
+      // it - 2 is full, every promotion warp has released it - 4, whose slot takes the scales of it + 4.
+      const uint32_t mine = pair < items ? (items - 1 - pair) / pairs + 1 : 0;
+      const uint64_t total = (uint64_t)mine * g.k_blocks;
+      uint32_t item = pair, kb = 0, row = 0, tile = 0;
+      uint64_t next = 0;                                // K-block whose scales are asked for next
+      auto load = [&]() {
+        if (next < total) {
+          if (kb == 0) {
+            uint32_t mt, nt;
+            pair_item(item, g.m_tiles, g.n_tiles, mt, nt);
+            row = mt * 256 + rank * 128 + lane;
+            tile = nt * 2 + (lane & 1);
+          }
+          const uint32_t slot = smem_u32(scales + (next % C::kScaleSlots) * C::kScaleSlotFloats);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            cp_async_f32(slot + (lane + 32 * j) * 4, g.a_scale + (uint64_t)min(row + 32 * j, g.m - 1) * g.a_scale_row + kb * g.a_scale_block);
+          if (lane < 2) cp_async_f32(slot + (128 + lane) * 4, g.w_scale + (uint64_t)min(tile, (g.n - 1) / kBlock) * g.w_scale_col + kb * g.w_scale_block);
+          if (++kb == g.k_blocks) { kb = 0; item += pairs; }
+        }
+        ++next;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      for (int j = 0; j < 4; ++j) load();
+      for (uint64_t it = 0; it < total; ++it) {
+        const uint32_t a = (uint32_t)it & 1;
+        if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (uint32_t)((it >> 1) & 1) ^ 1, abort_flag))) {
+          g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; break;
+        }
+        load();
+        asm volatile("cp.async.wait_group 4;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&tfull_bar[a]));
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairRegsHigh));
@@ -175,26 +220,18 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
       uint32_t mt, nt;
       pair_item(item, g.m_tiles, g.n_tiles, mt, nt);
       const uint32_t row0 = mt * 256 + rank * 128 + quad * 32, col0 = nt * 256 + wg * 64;
-      const float* sa_ptr = g.a_scale + (uint64_t)min(row0 + lane, g.m - 1) * g.a_scale_row;
-      const float* sw_ptr = g.w_scale + (uint64_t)(min(col0, g.n - 1) / kBlock) * g.w_scale_col;
       float2 acc[32];
 #pragma unroll
       for (int c = 0; c < 32; ++c) acc[c] = make_float2(0.0f, 0.0f);
-      // the scales of the next two K-blocks are on their way while one is being promoted
-      float sa0 = __ldg(sa_ptr), sw0 = __ldg(sw_ptr);
-      const uint32_t second = min(1u, g.k_blocks - 1);
-      float sa1 = __ldg(sa_ptr + second * g.a_scale_block), sw1 = __ldg(sw_ptr + second * g.w_scale_block);
       for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
         const uint32_t a = it & 1;
-        const float s = __fmul_rn(sa0, sw0);
-        const uint32_t ahead = min(kb + 2, g.k_blocks - 1);
-        sa0 = sa1; sw0 = sw1;
-        sa1 = __ldg(sa_ptr + ahead * g.a_scale_block); sw1 = __ldg(sw_ptr + ahead * g.w_scale_block);
         if (ok && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (it >> 1) & 1, abort_flag))) {
           g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; ok = false;
         }
         if (!ok) continue;
         tc_fence_after();
+        const float* slot = scales + (it % C::kScaleSlots) * C::kScaleSlotFloats;
+        const float s = __fmul_rn(slot[quad * 32 + lane], slot[128 + (wg >> 1)]);
         const float2 s2 = make_float2(s, s);
         uint32_t v[32];
         tmem_ld32_nowait(tbase + a * 256, v);
