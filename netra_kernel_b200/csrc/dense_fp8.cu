@@ -376,14 +376,22 @@ int dense_setup(int* sms, bool* pair_ok) {
       e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<128>::kSmemBytes);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(netra_dense_fp8_matmul_sm100<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DnCfg<128>::kSmemBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(netra_dense_fp8_pair_sm100<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(netra_dense_fp8_pair_sm100<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes);
     // the register re-balancing inside the pair kernels is only deadlock-free for the launch allocation it was written for
-    cudaFuncAttributes plain, transposed;
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&plain, netra_dense_fp8_pair_sm100<false>);
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&transposed, netra_dense_fp8_pair_sm100<true>);
+    bool ok = true;
+    auto pair = [&](const void* kernel) {
+      cudaFuncAttributes a;
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes);
+      if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, kernel);
+      if (e == cudaSuccess) ok = ok && a.numRegs == kPairRegsLaunch;
+    };
+    pair((const void*)netra_dense_fp8_pair_sm100<false, __nv_bfloat16>);
+    pair((const void*)netra_dense_fp8_pair_sm100<false, __half>);
+    pair((const void*)netra_dense_fp8_pair_sm100<false, float>);
+    pair((const void*)netra_dense_fp8_pair_sm100<true, __nv_bfloat16>);
+    pair((const void*)netra_dense_fp8_pair_sm100<true, __half>);
+    pair((const void*)netra_dense_fp8_pair_sm100<true, float>);
     if (e != cudaSuccess) return fail_cuda("dense set-up", e);
-    g_dense_pair_ok[device] = plain.numRegs == kPairRegsLaunch && transposed.numRegs == kPairRegsLaunch;
+    g_dense_pair_ok[device] = ok;
     g_dense_sms[device] = count;
   }
   *sms = g_dense_sms[device];
@@ -457,7 +465,7 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
     p.a_scale = a_scale_f32; p.a_scale_row = a_scale_row_stride; p.a_scale_block = a_scale_block_stride;
     p.w_scale = w_scale_f32;
     p.w_scale_col = transpose_w ? 1 : w_scale_pitch; p.w_scale_block = transpose_w ? w_scale_pitch : 1;
-    p.out = out; p.out_pitch = out_pitch; p.out_dtype = out_dtype;
+    p.out = out; p.out_pitch = out_pitch;
     p.m = m; p.n = n; p.k_blocks = (k + 127) / 128; p.m_tiles = (uint32_t)m256; p.n_tiles = (uint32_t)n256;
     const uint32_t size = (uint32_t)dense_element_bytes(out_dtype);
     p.tma_store = (uintptr_t)out % 16 == 0 && out_pitch * size % 16 == 0;
@@ -466,8 +474,14 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
     if (p.tma_store)
       if (int rc = encode_output(&tm_out, out, m, n, out_pitch, size)) return rc;
     const uint64_t pairs = m256 * n256 < (uint64_t)(sms / 2) ? m256 * n256 : (uint64_t)(sms / 2);
-    if (transpose_w) netra_dense_fp8_pair_sm100<true><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
-    else netra_dense_fp8_pair_sm100<false><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
+    auto launch = [&](auto element) {
+      using T = decltype(element);
+      if (transpose_w) netra_dense_fp8_pair_sm100<true, T><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
+      else netra_dense_fp8_pair_sm100<false, T><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
+    };
+    if (out_dtype == kDenseF32) launch(0.0f);
+    else if (out_dtype == kDenseF16) launch(__half{});
+    else launch(__nv_bfloat16{});
     return check_launch("dense_fp8_matmul launch");
   }
   DnArgs g;

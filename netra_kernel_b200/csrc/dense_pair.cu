@@ -6,7 +6,8 @@
 // time) and the promotion (128 KB read out of TMEM and 32,768 multiply-adds per CTA).  Sixteen promotion warps, four per
 // scheduler, hide the latencies of that chain that eight cannot; a thread keeps 64 columns of its row.
 //   warp 0: TMA producer (each CTA its own 128 rows and its own 128 weight rows; both report to the leader's barrier)
-//   warp 1: MMA issuer (leader CTA only; owns TMEM), warp 2: scales, warp 3: idle, warps 4..19: promotion and store
+//   warps 1 and 3: MMA issuers (leader CTA) or the relay of the peer's releases (warp 1, which also owns TMEM), warp 2: scales,
+//   warps 4..19: promotion and store
 // The scales go through shared memory, four K-blocks ahead: loaded by the promotion warps themselves, one K-block ahead, they
 // were what the loop waited for (785 ns a K-block against 600 with the loads dropped).
 // The grid is persistent; the accumulators are double-buffered in TMEM, so the next item's first two K-blocks run while an
@@ -35,7 +36,6 @@ struct PairArgs {
   uint64_t w_scale_col, w_scale_block;
   void* out;
   uint64_t out_pitch;
-  uint32_t out_dtype;
   uint32_t tma_store;                     // rows of the output start on 16-byte boundaries
   uint32_t m, n, k_blocks;
   uint32_t m_tiles, n_tiles;              // of 256
@@ -48,8 +48,34 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 }
 // Arrival on a barrier of either CTA of the pair.  It hands over TMEM columns, whose reads tcgen05.wait::ld has completed and
 // tcgen05.fence orders; no other memory is handed over.
-__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// one look at a barrier by a whole warp
+__device__ __forceinline__ bool mbar_try_wait_warp(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred p, p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+    if (mbar_try_wait_warp(bar, parity)) return true;
+    if ((spin & 0xff) == 0xff && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint32_t v[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 __device__ __forceinline__ void cp_async_f32(uint32_t dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -90,7 +116,7 @@ __device__ __forceinline__ void pair_item(uint32_t i, uint32_t m_tiles, uint32_t
   nt = j / rows;
 }
 
-template <bool kTransposed>
+template <bool kTransposed, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                            const __grid_constant__ CUtensorMap tm_out, const PairArgs g) {
@@ -100,9 +126,8 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   uint8_t* staging = smem + C::kStages * C::kStageBytes;
   float* scales = reinterpret_cast<float*>(staging + C::kStagingBytes);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kScaleSlots * C::kScaleSlotFloats);
-  uint64_t* empty_bar = full_bar + C::kStages;
-  uint64_t* tfull_bar = empty_bar + C::kStages;       // [2]
-  uint64_t* tempty_bar = tfull_bar + 2;               // [2]
+  uint64_t* done_bar = full_bar + C::kStages;         // a stage's MMAs are done and its scales are there
+  uint64_t* tempty_bar = done_bar + C::kStages;       // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
@@ -111,8 +136,8 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   const uint32_t items = g.m_tiles * g.n_tiles, pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 2); mbar_init(smem_u32(&tempty_bar[a]), 32); }
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&done_bar[s]), 2); }
+    for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&tempty_bar[a]), rank == 0 ? 17 : 16);   // promotion warps, and the peer's relay
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -139,7 +164,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
         const int row = (int)(mt * 256 + rank * 128), col = (int)(nt * 256 + rank * 128);
         for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
           const uint32_t s = it % C::kStages;
-          if (!mbar_wait(smem_u32(&empty_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
+          if (!mbar_wait(smem_u32(&done_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
             g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; ok = false; break;
           }
           if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * C::kStageBytes);
@@ -149,27 +174,36 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
           else tma_load_2d_pair(dst + 128 * kBlock, &tm_w, bar, (int)(kb * kBlock), col, pol);
         }
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if ((warp == 1 || warp == 3) && lane == 0 && rank == 0) {
+      // Two threads take alternate K-blocks, each its own accumulator stage: while one feeds its four MMAs to the tensor pipe,
+      // the other is already through its waits.  The operands, which are early, are waited for first.
       const uint32_t idesc = (1u << 4) | (kTransposed ? 1u << 16 : 0u) | ((256u >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
-      uint32_t it = 0;
-      bool ok = true;
-      for (uint32_t item = pair; ok && item < items; item += pairs) {
-        for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
-          const uint32_t s = it % C::kStages, a = it & 1;
-          if (!mbar_wait(smem_u32(&tempty_bar[a]), ((it >> 1) & 1) ^ 1, abort_flag) ||
-              !mbar_wait(smem_u32(&full_bar[s]), (it / C::kStages) & 1, abort_flag)) {
-            g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; ok = false; break;
-          }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
-          const uint64_t adesc = make_smem_desc(sa);
-          const uint64_t bdesc = kTransposed ? make_smem_desc_mn(sa + 128 * kBlock) : make_smem_desc(sa + 128 * kBlock);
-#pragma unroll
-          for (int k = 0; k < kBlock / 32; ++k)
-            umma_f8_pair(tmem_base + a * 256, adesc + 2 * k, bdesc + (kTransposed ? 256 : 2) * k, idesc, k > 0);
-          umma_commit_pair(smem_u32(&empty_bar[s]));
-          umma_commit_pair(smem_u32(&tfull_bar[a]));
+      const uint32_t a = (uint32_t)warp >> 1, mine = pair < items ? (items - 1 - pair) / pairs + 1 : 0;
+      const uint64_t total = (uint64_t)mine * g.k_blocks;
+      uint32_t phase = 1;
+      for (uint64_t it = a; it < total; it += 2, phase ^= 1) {
+        const uint32_t s = (uint32_t)it % C::kStages;
+        if (!mbar_wait(smem_u32(&full_bar[s]), (uint32_t)(it / C::kStages) & 1, abort_flag) ||
+            !mbar_wait(smem_u32(&tempty_bar[a]), phase, abort_flag)) {
+          g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break;
         }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
+        const uint64_t adesc = make_smem_desc(sa);
+        const uint64_t bdesc = kTransposed ? make_smem_desc_mn(sa + 128 * kBlock) : make_smem_desc(sa + 128 * kBlock);
+#pragma unroll
+        for (int k = 0; k < kBlock / 32; ++k)
+          umma_f8_pair(tmem_base + a * 256, adesc + 2 * k, bdesc + (kTransposed ? 256 : 2) * k, idesc, k > 0);
+        umma_commit_pair(smem_u32(&done_bar[s]));
+      }
+    } else if (warp == 1 && lane == 0) {
+      // The peer's sixteen releases reach the leader as one arrival.
+      const uint32_t mine = pair < items ? (items - 1 - pair) / pairs + 1 : 0;
+      const uint64_t total = (uint64_t)mine * g.k_blocks;
+      for (uint64_t it = 0; it < total; ++it) {
+        const uint32_t a = (uint32_t)it & 1;
+        if (!mbar_wait(smem_u32(&tempty_bar[a]), (uint32_t)(it >> 1) & 1, abort_flag)) { g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break; }
+        mbar_arrive_peer(map_to_rank(smem_u32(&tempty_bar[a]), 0));
       }
     } else if (warp == 2) {
       // An accumulator stage counts as full when its MMAs are done and its K-block's scales are in their slot.  Once K-block
@@ -198,96 +232,104 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
       };
       for (int j = 0; j < 4; ++j) load();
       for (uint64_t it = 0; it < total; ++it) {
-        const uint32_t a = (uint32_t)it & 1;
-        if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (uint32_t)((it >> 1) & 1) ^ 1, abort_flag))) {
+        if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&done_bar[(it - 2) % C::kStages]), (uint32_t)((it - 2) / C::kStages) & 1, abort_flag))) {
           g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; break;
         }
         load();
         asm volatile("cp.async.wait_group 4;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&tfull_bar[a]));
+        if (lane == 0) mbar_arrive(smem_u32(&done_bar[it % C::kStages]));
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairRegsHigh));
     const int wg = (warp - 4) >> 2, quad = warp & 3;            // 64 columns and 32 rows of this warp
-    uint8_t* tile = staging + (warp - 4) * 4096;
-    const uint32_t tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(wg * 64);
-    uint32_t it = 0;
+    const uint32_t tile = smem_u32(staging) + (uint32_t)(warp - 4) * 4096u, my_row = tile + (uint32_t)lane * 128u;
+    // This loop is paced by the instructions its sixteen warps issue (four per scheduler), so what can be carried from one
+    // K-block to the next is carried: the barrier's address and phase, the scales' slot (four stages and two phases make the
+    // eight slots), the TMEM column of the accumulator stage.
+    const uint32_t bar0 = smem_u32(&done_bar[0]);
+    const uint32_t slot0 = smem_u32(scales) + (uint32_t)(quad * 32 + lane) * 4u, tile_scale = (uint32_t)(128 + (wg >> 1) - (quad * 32 + lane)) * 4u;
+    uint32_t stage = 0, phase = 0, column = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(wg * 64);
+    static_assert(C::kScaleSlots == 2 * C::kStages, "a slot is a stage and the parity of its phase");
+    const bool first_lane = lane == 0;
+    uint32_t release = smem_u32(&tempty_bar[0]);
     bool ok = true;
-    for (uint32_t item = pair; item < items; item += pairs) {
+    for (uint32_t item = pair; ok && item < items; item += pairs) {
       uint32_t mt, nt;
       pair_item(item, g.m_tiles, g.n_tiles, mt, nt);
       const uint32_t row0 = mt * 256 + rank * 128 + quad * 32, col0 = nt * 256 + wg * 64;
       float2 acc[32];
 #pragma unroll
       for (int c = 0; c < 32; ++c) acc[c] = make_float2(0.0f, 0.0f);
-      for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
-        const uint32_t a = it & 1;
-        if (ok && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (it >> 1) & 1, abort_flag))) {
-          g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; ok = false;
-        }
-        if (!ok) continue;
+#pragma unroll 1
+      for (uint32_t kb = 0; kb < g.k_blocks; ++kb) {
+        const uint32_t bar = bar0 + 8 * stage;
+        if (!mbar_wait_warp(bar, phase, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        const float* slot = scales + (it % C::kScaleSlots) * C::kScaleSlotFloats;
-        const float s = __fmul_rn(slot[quad * 32 + lane], slot[128 + (wg >> 1)]);
-        const float2 s2 = make_float2(s, s);
         uint32_t v[32];
-        tmem_ld32_nowait(tbase + a * 256, v);
+        tmem_ld32_nowait(column, v);
+        const uint32_t slot = slot0 + (stage + phase * C::kStages) * (C::kScaleSlotFloats * 4);
+        const float s = __fmul_rn(ld_shared_f32(slot), ld_shared_f32(slot + tile_scale));
+        const float2 s2 = make_float2(s, s);
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), s2, acc[c]);
-        tmem_ld32_nowait(tbase + a * 256 + 32, v);
+        tmem_ld32_nowait(column + 32, v);
+        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_pair(map_to_rank(smem_u32(&tempty_bar[a]), 0));
+        if (first_lane) mbar_arrive(release);
+        release ^= 8;
+        column ^= 256;
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[16 + c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), s2, acc[16 + c]);
       }
+      if (!ok) { g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; break; }
       // ---- store: 128 bytes per row at a time through this warp's own staging rows (chunk j of row r at j ^ (r & 7), the
       // 128-byte swizzle of the copy engine), 64 columns of a 16-bit type or 32 of FP32
-      const bool wide = g.out_dtype == kDenseF32;
-      const uint32_t per_pass = wide ? 32 : 64;
+      constexpr int kPasses = sizeof(T) / 2, kPassCols = 64 / kPasses;
 #pragma unroll
-      for (int pass = 0; pass < 2; ++pass) {
-        if (pass == 1 && !wide) break;
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the last copy has left the rows
+      for (int pass = 0; pass < kPasses; ++pass) {
+        if (first_lane) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the last copy has left the rows
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint32_t p[4];
-          if (wide) {
+          if constexpr (kPasses == 2) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) { const float2 f = acc[pass * 16 + 2 * j + q]; p[2 * q] = __float_as_uint(f.x); p[2 * q + 1] = __float_as_uint(f.y); }
           } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const float2 f = acc[4 * j + q];
-              if (g.out_dtype == kDenseF16) { const __half2 h = __floats2half2_rn(f.x, f.y); p[q] = *reinterpret_cast<const uint32_t*>(&h); }
+              if constexpr (std::is_same<T, __half>::value) { const __half2 h = __floats2half2_rn(f.x, f.y); p[q] = *reinterpret_cast<const uint32_t*>(&h); }
               else { const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y); p[q] = *reinterpret_cast<const uint32_t*>(&h); }
             }
           }
-          *reinterpret_cast<uint4*>(tile + lane * 128 + 16 * (j ^ (lane & 7))) = make_uint4(p[0], p[1], p[2], p[3]);
+          st_shared_v4(my_row + 16 * (j ^ (lane & 7)), p);
         }
-        const uint32_t col = col0 + pass * 32;
+        const uint32_t col = col0 + pass * kPassCols;
         if (g.tma_store) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) {
-            if (row0 < g.m && col < g.n) tma_store_2d(&tm_out, smem_u32(tile), (int)col, (int)row0);
+          if (first_lane) {
+            if (row0 < g.m && col < g.n) tma_store_2d(&tm_out, tile, (int)col, (int)row0);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
         } else {
+          // rows that do not start on 16-byte boundaries: a lane a column
           __syncwarp();
+          T* out = reinterpret_cast<T*>(g.out);
+          const uint8_t* rows = staging + (warp - 4) * 4096;
+#pragma unroll 1
           for (uint32_t r = 0; r < 32 && row0 + r < g.m; ++r)
-            for (uint32_t c = lane; c < per_pass && col + c < g.n; c += 32) {
-              const uint32_t byte = c * (wide ? 4 : 2);
-              const uint8_t* src = tile + r * 128 + 16 * ((byte >> 4) ^ (r & 7)) + (byte & 15);
-              const uint64_t at = (uint64_t)(row0 + r) * g.out_pitch + col + c;
-              if (wide) reinterpret_cast<uint32_t*>(g.out)[at] = *reinterpret_cast<const uint32_t*>(src);
-              else reinterpret_cast<uint16_t*>(g.out)[at] = *reinterpret_cast<const uint16_t*>(src);
+#pragma unroll 1
+            for (uint32_t c = lane; c < (uint32_t)kPassCols && col + c < g.n; c += 32) {
+              const uint32_t byte = c * (uint32_t)sizeof(T);
+              out[(uint64_t)(row0 + r) * g.out_pitch + col + c] = *reinterpret_cast<const T*>(rows + r * 128 + 16 * ((byte >> 4) ^ (r & 7)) + (byte & 15));
             }
           __syncwarp();
         }
