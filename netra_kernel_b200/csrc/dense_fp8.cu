@@ -27,6 +27,11 @@ __device__ __forceinline__ void dense_store(void* p, uint32_t dtype, size_t i, f
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
+// The product may be launched while the kernel before it is still running (programmatic dependent launch): the set-up of its
+// barriers and TMEM overlaps that kernel's end, and every access to global memory comes after the wait.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ------------------------------------------------------------------------------------------
 // Row quantiser.  Sixteen lanes own one block of 128 columns of kRows neighbouring rows, eight neighbouring columns each: a
 // BF16 lane loads 16 bytes and stores 8 codes.  HBM bound; the four rows of the large form keep four loads in flight per
@@ -64,6 +69,7 @@ template <typename T, bool kVector, int kRows>
 __global__ void __launch_bounds__(256)
 netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8_t* __restrict__ codes, uint64_t codes_pitch,
                                 float* __restrict__ scale, uint64_t scale_row, uint64_t scale_block, uint32_t m, uint32_t k) {
+  grid_dependency_trigger();
   const uint32_t blocks = (k + kBlock - 1) / kBlock;
   const uint32_t item = (blockIdx.x * 256u + threadIdx.x) >> 4;
   const uint32_t group = item / blocks, b = item - group * blocks;
@@ -148,7 +154,7 @@ struct DnArgs {
   uint64_t w_scale_col, w_scale_block;    // per 128 output columns, per K-block
   void* out;
   uint64_t out_pitch;
-  uint32_t out_dtype;
+  uint32_t out_dtype, out_vector;         // out_vector: four neighbouring elements are one aligned access
   uint32_t m, n, k_blocks;                // rows, output columns, K-blocks
   uint32_t n_tiles;
 };
@@ -172,6 +178,25 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
   return v;
+}
+
+// one look at a barrier by a whole warp
+__device__ __forceinline__ bool mbar_try_wait_warp(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred p, p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+    if (mbar_try_wait_warp(bar, parity)) return true;
+    if ((spin & 0xff) == 0xff && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  return false;
 }
 
 // MN-major, 128-byte-swizzled operand tile: 128 output columns (bytes) per row, one row per reduction index; groups of
@@ -215,6 +240,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_wait();                   // nothing above touches global memory
 
   if (warp == 0 && lane == 0) {
     const uint64_t pol = policy_evict_last();
@@ -253,25 +279,45 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
     float acc[kCols];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
-    float sa = kb0 < kb1 ? __ldg(sa_ptr + kb0 * g.a_scale_block) : 0.0f, sw = kb0 < kb1 ? __ldg(sw_ptr + kb0 * g.w_scale_block) : 0.0f;
-    for (uint32_t kb = kb0; kb < kb1; ++kb) {
-      const uint32_t it = kb - kb0, a = it % C::kAccStages;
-      const float s = __fmul_rn(sa, sw);
-      if (kb + 1 < kb1) { sa = __ldg(sa_ptr + (kb + 1) * g.a_scale_block); sw = __ldg(sw_ptr + (kb + 1) * g.w_scale_block); }
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull_bar[a]), (it / C::kAccStages) & 1, abort_flag))) { g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; break; }
-      tc_fence_after();
-      const uint32_t t = tmem_base + ((uint32_t)(quad * 32) << 16) + a * kBN + wg * kCols;
-      uint32_t v[kCols / 32][32];
+    // scales of eight K-blocks at a time, the next eight on their way: one at a time, their latency set the loop's pace
+    float s[8], ahead[8];
 #pragma unroll
-      for (int q = 0; q < kCols / 32; ++q) tmem_ld32_nowait(t + 32 * q, v[q]);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[a]));
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t kb = min(kb0 + j, g.k_blocks - 1);
+      s[j] = __ldcg(sa_ptr + kb * g.a_scale_block) * __ldcg(sw_ptr + kb * g.w_scale_block);
+    }
+    bool ok = true;
+    for (uint32_t base = kb0; ok && base < kb1; base += 8) {
+      if (base + 8 < kb1) {
 #pragma unroll
-      for (int q = 0; q < kCols / 32; ++q)
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t kb = min(base + 8 + j, g.k_blocks - 1);
+          ahead[j] = __ldcg(sa_ptr + kb * g.a_scale_block) * __ldcg(sw_ptr + kb * g.w_scale_block);
+        }
+      }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) acc[32 * q + c] = fmaf(__uint_as_float(v[q][c]), s, acc[32 * q + c]);
+      for (int j = 0; j < 8; ++j) {
+        if (!ok || base + j >= kb1) break;
+        const uint32_t it = base + j - kb0, a = it % C::kAccStages;
+        if (!mbar_wait_warp(smem_u32(&tfull_bar[a]), (it / C::kAccStages) & 1, abort_flag)) {
+          g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; ok = false; break;
+        }
+        tc_fence_after();
+        const uint32_t t = tmem_base + ((uint32_t)(quad * 32) << 16) + a * kBN + wg * kCols;
+        uint32_t v[kCols / 32][32];
+#pragma unroll
+        for (int q = 0; q < kCols / 32; ++q) tmem_ld32_nowait(t + 32 * q, v[q]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[a]));
+#pragma unroll
+        for (int q = 0; q < kCols / 32; ++q)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) acc[32 * q + c] = fmaf(__uint_as_float(v[q][c]), s[j], acc[32 * q + c]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = ahead[j];
     }
     __syncwarp();
     // every MMA of this CTA has completed (the last accumulator stage was waited for), so the stages are free
@@ -291,23 +337,39 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   }
   __syncwarp();
   if (ranks > 1) cluster_barrier();
-  // rows r = rank, rank + ranks, ... ; a warp takes a row, a lane four neighbouring columns at a time
-  const uint32_t base = smem_u32(smem);
-  for (uint32_t i = warp; i * ranks + rank < 128u; i += kDnThreads / 32) {
+  // rows r = rank, rank + ranks, ... ; a quarter, half or whole warp takes a row, a lane four neighbouring columns
+  constexpr uint32_t kLanes = kBN / 4, kRowsAtOnce = (kDnThreads / 32) * (32 / kLanes);
+  const uint32_t base = smem_u32(smem), c = (threadIdx.x % kLanes) * 4, col = col0 + c;
+#pragma unroll 2
+  for (uint32_t i = threadIdx.x / kLanes; i * ranks + rank < 128u; i += kRowsAtOnce) {
     const uint32_t r = i * ranks + rank, row = row0 + r;
-    if (row >= g.m) break;
-    for (uint32_t c = lane * 4; c < (uint32_t)kBN; c += 128) {
-      if (col0 + c >= g.n) break;
-      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (uint32_t j = 0; j < ranks; ++j) {
-        const uint32_t addr = base + (r * C::kOutPitch + c) * 4;
-        const float4 p = ld_cluster_f4(addr, j);
-        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+    if (row >= g.m || col >= g.n) continue;
+    const uint32_t addr = base + (r * C::kOutPitch + c) * 4;
+    float4 sum = ld_cluster_f4(addr, 0);
+    for (uint32_t j = 1; j < ranks; ++j) {
+      const float4 p = ld_cluster_f4(addr, j);
+      sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+    }
+    const uint64_t at = (uint64_t)row * g.out_pitch + col;
+    if (g.out_vector && col + 4 <= g.n) {
+      if (g.out_dtype == kDenseF32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at) = sum;
+      } else {
+        uint2 p;
+        if (g.out_dtype == kDenseF16) {
+          const __half2 lo = __floats2half2_rn(sum.x, sum.y), hi = __floats2half2_rn(sum.z, sum.w);
+          p = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+          p = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.out) + at) = p;
       }
+    } else {
       const float o[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col0 + c + j < g.n) dense_store(g.out, g.out_dtype, (uint64_t)row * g.out_pitch + col0 + c + j, o[j]);
+        if (col + j < g.n) dense_store(g.out, g.out_dtype, at + j, o[j]);
     }
   }
   __syncwarp();
@@ -317,6 +379,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
 }  // namespace netra
 
 #include "dense_pair.cu"
+#include "dense_few.cu"
 
 namespace {
 
@@ -400,7 +463,54 @@ int dense_setup(int* sms, bool* pair_ok) {
 }
 
 constexpr uint32_t kDenseMaxSize = 1u << 26;
+constexpr uint32_t kFewMaxRows = 16, kFewMaxCodeRows = 32;
 
+// Product of few rows; x of type code `source` (kDense*, or 3 for codes with their scales).
+int launch_few(const FewArgs& g, uint32_t source, cudaStream_t stream) {
+  const uint32_t blocks = (g.k + 127) / 128, warps = blocks < 2 ? 1 : blocks / 2 < 16 ? (blocks + 1) / 2 : 16;
+  const uint32_t tiles = g.m <= 8 ? 1 : g.m <= 16 ? 2 : 4;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((g.n + kFewRows - 1) / kFewRows); cfg.blockDim = dim3(32 * warps);
+  cfg.dynamicSmemBytes = warps * tiles * 8 * kFewRows * sizeof(float);
+  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
+  auto launch = [&](auto element) {
+    using T = decltype(element);
+    if constexpr (sizeof(T) == 1) {
+      if (tiles == 4) return cudaLaunchKernelEx(&cfg, netra_dense_fp8_few_sm100<T, 4>, g);
+    }
+    return tiles == 1 ? cudaLaunchKernelEx(&cfg, netra_dense_fp8_few_sm100<T, 1>, g) : cudaLaunchKernelEx(&cfg, netra_dense_fp8_few_sm100<T, 2>, g);
+  };
+  const cudaError_t e = source == 3 ? launch((uint8_t)0) : source == kDenseF32 ? launch(0.0f) : source == kDenseF16 ? launch(__half{}) : launch(__nv_bfloat16{});
+  return e == cudaSuccess ? check_launch("dense_fp8 launch (few rows)") : fail_cuda("dense_fp8 launch (few rows)", e);
+}
+
+
+int check_quantize_operands(const void* x, uint32_t dtype, uint64_t x_pitch, uint32_t m, uint32_t k) {
+  if (!x) return fail("dense_quantize_rows: null pointer");
+  if (dtype > kDenseF32) return fail("dense_quantize_rows: unknown element type");
+  if (m == 0 || k == 0 || m > kDenseMaxSize || k > kDenseMaxSize) return fail("dense_quantize_rows: rows and columns must be 1..2^26");
+  if (m > 1 && x_pitch < k) return fail("dense_quantize_rows: a row pitch is smaller than the row");
+  if ((uintptr_t)x % dense_element_bytes(dtype)) return fail("dense_quantize_rows: input is not aligned to its element");
+  return 0;
+}
+
+int check_matmul_operands(const void* out, uint32_t out_dtype, uint64_t out_pitch, const void* w, uint64_t w_pitch, const float* w_scale,
+                          uint64_t w_scale_pitch, uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols) {
+  if (!out || !w || !w_scale) return fail("dense_fp8_matmul: null pointer");
+  if (out_dtype > kDenseF32) return fail("dense_fp8_matmul: unknown element type");
+  if (transpose_w > 1) return fail("dense_fp8_matmul: transpose_w must be 0 or 1");
+  if (m == 0 || w_rows == 0 || w_cols == 0 || m > kDenseMaxSize || w_rows > kDenseMaxSize || w_cols > kDenseMaxSize)
+    return fail("dense_fp8_matmul: sizes must be 1..2^26");
+  if (w_pitch % 16 || (uintptr_t)w % 16) return fail("dense_fp8_matmul: codes need 16-byte aligned addresses and row pitches");
+  if (w_pitch < w_cols || out_pitch < (transpose_w ? w_cols : w_rows) || w_scale_pitch < (w_cols + 127) / 128)
+    return fail("dense_fp8_matmul: a row pitch is smaller than the row");
+  if ((uintptr_t)out % dense_element_bytes(out_dtype) || (uintptr_t)w_scale % 4)
+    return fail("dense_fp8_matmul: an address is not aligned to its element");
+  return 0;
+}
 
 }  // namespace
 
@@ -409,11 +519,9 @@ extern "C" {
 int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, float* scale_f32, uint64_t scale_row_stride,
                                      uint64_t scale_block_stride, const void* x, uint32_t x_dtype, uint64_t x_pitch, uint32_t m,
                                      uint32_t k, cudaStream_t stream) {
-  if (!codes_fp8 || !scale_f32 || !x) return fail("dense_quantize_rows: null pointer");
-  if (x_dtype > kDenseF32) return fail("dense_quantize_rows: unknown element type");
-  if (m == 0 || k == 0 || m > kDenseMaxSize || k > kDenseMaxSize) return fail("dense_quantize_rows: rows and columns must be 1..2^26");
-  if ((m > 1 && x_pitch < k) || (m > 1 && codes_pitch < k)) return fail("dense_quantize_rows: a row pitch is smaller than the row");
-  if ((uintptr_t)x % dense_element_bytes(x_dtype)) return fail("dense_quantize_rows: input is not aligned to its element");
+  if (!codes_fp8 || !scale_f32) return fail("dense_quantize_rows: null pointer");
+  if (int rc = check_quantize_operands(x, x_dtype, x_pitch, m, k)) return rc;
+  if (m > 1 && codes_pitch < k) return fail("dense_quantize_rows: a row pitch is smaller than the row");
   const uint64_t blocks = (k + 127) / 128;
   // four rows per lane once that still leaves every SM a few thousand lanes; below, one row each for the shortest chain
   const bool deep = (uint64_t)m * blocks >= 32768;
@@ -441,21 +549,20 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
                                   const float* a_scale_f32, uint64_t a_scale_row_stride, uint64_t a_scale_block_stride,
                                   const void* w_fp8, uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch,
                                   uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols, cudaStream_t stream) {
-  if (!out || !a_fp8 || !a_scale_f32 || !w_fp8 || !w_scale_f32) return fail("dense_fp8_matmul: null pointer");
-  if (out_dtype > kDenseF32) return fail("dense_fp8_matmul: unknown element type");
-  if (transpose_w > 1) return fail("dense_fp8_matmul: transpose_w must be 0 or 1");
-  if (m == 0 || w_rows == 0 || w_cols == 0 || m > kDenseMaxSize || w_rows > kDenseMaxSize || w_cols > kDenseMaxSize)
-    return fail("dense_fp8_matmul: sizes must be 1..2^26");
+  if (!a_fp8 || !a_scale_f32) return fail("dense_fp8_matmul: null pointer");
+  if (int rc = check_matmul_operands(out, out_dtype, out_pitch, w_fp8, w_pitch, w_scale_f32, w_scale_pitch, transpose_w, m, w_rows, w_cols)) return rc;
   const uint32_t n = transpose_w ? w_cols : w_rows, k = transpose_w ? w_rows : w_cols;
-  if (a_pitch % 16 || w_pitch % 16 || (uintptr_t)a_fp8 % 16 || (uintptr_t)w_fp8 % 16)
-    return fail("dense_fp8_matmul: codes need 16-byte aligned addresses and row pitches");
-  if (a_pitch < k || w_pitch < w_cols || out_pitch < n || w_scale_pitch < (w_cols + 127) / 128)
-    return fail("dense_fp8_matmul: a row pitch is smaller than the row");
-  if ((uintptr_t)out % dense_element_bytes(out_dtype) || (uintptr_t)a_scale_f32 % 4 || (uintptr_t)w_scale_f32 % 4)
-    return fail("dense_fp8_matmul: an address is not aligned to its element");
+  if (a_pitch % 16 || (uintptr_t)a_fp8 % 16) return fail("dense_fp8_matmul: codes need 16-byte aligned addresses and row pitches");
+  if (a_pitch < k) return fail("dense_fp8_matmul: a row pitch is smaller than the row");
+  if ((uintptr_t)a_scale_f32 % 4) return fail("dense_fp8_matmul: an address is not aligned to its element");
   int sms = 0;
   bool pair_ok = false;
   if (int rc = dense_setup(&sms, &pair_ok)) return rc;
+  if (!transpose_w && m <= kFewMaxCodeRows) {
+    const FewArgs f = {a_fp8, a_pitch, a_scale_f32, a_scale_row_stride, a_scale_block_stride, (const uint8_t*)w_fp8, w_pitch, w_scale_f32,
+                       w_scale_pitch, out, out_pitch, out_dtype, m, n, k};
+    return launch_few(f, 3, stream);
+  }
   CUtensorMap tm_a, tm_w;
   if (int rc = encode_codes(&tm_a, a_fp8, m, k, a_pitch, 128)) return rc;
   const uint64_t m256 = (m + 255) / 256, n256 = (n + 255) / 256;
@@ -474,15 +581,19 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
     if (p.tma_store)
       if (int rc = encode_output(&tm_out, out, m, n, out_pitch, size)) return rc;
     const uint64_t pairs = m256 * n256 < (uint64_t)(sms / 2) ? m256 * n256 : (uint64_t)(sms / 2);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = PairCfg::kSmemBytes;
+    cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
     auto launch = [&](auto element) {
       using T = decltype(element);
-      if (transpose_w) netra_dense_fp8_pair_sm100<true, T><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
-      else netra_dense_fp8_pair_sm100<false, T><<<(unsigned)(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream>>>(tm_a, tm_w, tm_out, p);
+      return transpose_w ? cudaLaunchKernelEx(&cfg, netra_dense_fp8_pair_sm100<true, T>, tm_a, tm_w, tm_out, p)
+                         : cudaLaunchKernelEx(&cfg, netra_dense_fp8_pair_sm100<false, T>, tm_a, tm_w, tm_out, p);
     };
-    if (out_dtype == kDenseF32) launch(0.0f);
-    else if (out_dtype == kDenseF16) launch(__half{});
-    else launch(__nv_bfloat16{});
-    return check_launch("dense_fp8_matmul launch");
+    const cudaError_t e = out_dtype == kDenseF32 ? launch(0.0f) : out_dtype == kDenseF16 ? launch(__half{}) : launch(__nv_bfloat16{});
+    return e == cudaSuccess ? check_launch("dense_fp8_matmul launch") : fail_cuda("dense_fp8_matmul launch", e);
   }
   DnArgs g;
   g.a_scale = a_scale_f32; g.a_scale_row = a_scale_row_stride; g.a_scale_block = a_scale_block_stride;
@@ -490,6 +601,7 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   g.w_scale_col = transpose_w ? 1 : w_scale_pitch;
   g.w_scale_block = transpose_w ? w_scale_pitch : 1;
   g.out = out; g.out_pitch = out_pitch; g.out_dtype = out_dtype;
+  g.out_vector = (uintptr_t)out % (4 * dense_element_bytes(out_dtype)) == 0 && out_pitch % 4 == 0;
   g.m = m; g.n = n; g.k_blocks = (k + 127) / 128;
   const uint64_t m_tiles = (m + 127) / 128;
   const bool narrow = !transpose_w && m_tiles * ((n + 127) / 128) * 2 <= (uint64_t)sms;
@@ -501,11 +613,13 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   if (tiles * split > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
   if (int rc = encode_codes(&tm_w, w_fp8, w_rows, w_cols, w_pitch, transpose_w ? 128 : bn)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(tiles * split)); cfg.blockDim = dim3(kDnThreads);
-  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
+  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 2;
   cudaError_t e;
   if (transpose_w) {
     cfg.dynamicSmemBytes = DnCfg<128>::kSmemBytes;
@@ -534,6 +648,16 @@ int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, 
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < netra_dense_fp8_linear_workspace_bytes(m, k))
     return fail("dense_fp8_linear: workspace missing, too small or not 16-byte aligned");
   const uint64_t pitch = ((uint64_t)k + 15) / 16 * 16;
+  // few rows: the product quantises them itself, if whole 16-byte accesses fit them
+  if (!transpose_w && m <= kFewMaxRows && k % 8 == 0 && (uintptr_t)x % 16 == 0 && x_pitch * dense_element_bytes(dtype) % 16 == 0) {
+    if (int rc = check_quantize_operands(x, dtype, x_pitch, m, k)) return rc;
+    if (int rc = check_matmul_operands(out, dtype, out_pitch, w_fp8, w_pitch, w_scale_f32, w_scale_pitch, transpose_w, m, w_rows, w_cols)) return rc;
+    int sms = 0;
+    bool pair_ok = false;
+    if (int rc = dense_setup(&sms, &pair_ok)) return rc;
+    const FewArgs f = {x, x_pitch, nullptr, 0, 0, (const uint8_t*)w_fp8, w_pitch, w_scale_f32, w_scale_pitch, out, out_pitch, dtype, m, w_rows, k};
+    return launch_few(f, dtype, stream);
+  }
   uint8_t* codes = (uint8_t*)workspace;
   float* scale = (float*)(codes + (uint64_t)m * pitch);
   if (int rc = netra_dense_quantize_rows_launch(codes, pitch, scale, 1, m, x, dtype, x_pitch, m, k, stream)) return rc;
