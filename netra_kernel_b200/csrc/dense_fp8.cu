@@ -127,9 +127,12 @@ netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8
 // ------------------------------------------------------------------------------------------
 // Product on the tensor cores.  A cluster owns 128 rows x kBN columns of the output and splits the K-blocks among
 // its CTAs; per K-block the raw sums leave TMEM and are promoted as acc = fma(part, sa * sw, acc), as in the grouped GEMMs.
-//   warp 0: TMA producer, warp 1: MMA issuer (owns TMEM), warps 4..11: promotion (two groups halve the columns)
-// At the end every CTA lays its FP32 partial tile into its shared memory and sums a share of the rows over the cluster
-// in rank order (deterministic).
+//   warps 0 and 2: TMA producers (rows, weight), warps 1 and 3: MMA issuers (alternate K-blocks; warp 1 owns TMEM),
+//   warps 4..11: promotion (two groups halve the columns)
+// With the few K-blocks a CTA has here, what costs is the chain of steps of one thread: a K-block took 750 cycles with one
+// producer and one issuer (two barrier waits, four MMAs, two commits), whatever the tile's width.
+// At the end every CTA hands each row of its FP32 partial tile to the cluster's CTA that owns the row (stores into that CTA's
+// shared memory), which adds the parts in rank order: deterministic, and one cluster barrier.
 // ------------------------------------------------------------------------------------------
 constexpr int kDnThreads = 384;
 
@@ -138,12 +141,13 @@ struct DnCfg {
   static constexpr int kABytes = 128 * kBlock;
   static constexpr int kBBytes = kBN * kBlock;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = kBN >= 128 ? 6 : 8;
-  static constexpr int kAccStages = 512 / kBN > 4 ? 4 : 512 / kBN;
+  static constexpr int kStages = kBN >= 128 ? 4 : 6;
+  static constexpr int kAccStages = 4;
+  static_assert(kStages >= kAccStages, "a stage's barrier may not run two phases ahead of the promotion");
   static constexpr int kTmemCols = kAccStages * kBN;
   static constexpr int kOutPitch = kBN + 4;            // floats; 16-byte row stores fall on different banks
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512;
-  static_assert(128 * kOutPitch * 4 <= kStages * kStageBytes, "the partial tile reuses the stages");
+  static constexpr int kOutBytes = 128 * kOutPitch * 4;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kOutBytes + 256;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of one SM");
 };
 
@@ -172,12 +176,15 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
-  return v;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
 // one look at a barrier by a whole warp
@@ -214,11 +221,10 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   static_assert(!kTransposed || kBN == 128, "a transposed weight tile is one 128-byte swizzle atom wide");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
-  uint64_t* full_bar = bars;
-  uint64_t* empty_bar = full_bar + C::kStages;
-  uint64_t* tfull_bar = empty_bar + C::kStages;
-  uint64_t* tempty_bar = tfull_bar + C::kAccStages;
+  float* parts = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);      // [ranks][128 / ranks rows][kOutPitch]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes + C::kOutBytes);
+  uint64_t* done_bar = full_bar + C::kStages;          // the MMAs that read the stage are done
+  uint64_t* tempty_bar = done_bar + C::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + C::kAccStages);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
@@ -229,8 +235,8 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   const uint32_t kb0 = (uint32_t)((uint64_t)g.k_blocks * rank / ranks), kb1 = (uint32_t)((uint64_t)g.k_blocks * (rank + 1) / ranks);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
-    for (int a = 0; a < C::kAccStages; ++a) { mbar_init(smem_u32(&tfull_bar[a]), 1); mbar_init(smem_u32(&tempty_bar[a]), 8); }
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&done_bar[s]), 1); }
+    for (int a = 0; a < C::kAccStages; ++a) mbar_init(smem_u32(&tempty_bar[a]), 8);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -240,25 +246,31 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (ranks > 1) cluster_arrive();          // this CTA is running: others may store into its shared memory
   grid_dependency_wait();                   // nothing above touches global memory
 
-  if (warp == 0 && lane == 0) {
+  if ((warp == 0 || warp == 2) && lane == 0) {
     const uint64_t pol = policy_evict_last();
+    const bool rows = warp == 0;
     for (uint32_t kb = kb0; kb < kb1; ++kb) {
       const uint32_t it = kb - kb0, s = it % C::kStages;
-      if (!mbar_wait(smem_u32(&empty_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) { g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; break; }
+      if (it >= C::kStages && !mbar_wait(smem_u32(&done_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
+        g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; break;
+      }
       const uint32_t bar = smem_u32(&full_bar[s]), dst = smem_u32(smem + s * C::kStageBytes);
-      mbar_expect_tx(bar, C::kStageBytes);
-      tma_load_2d(dst, &tm_a, bar, (int)(kb * kBlock), (int)row0, pol);
-      if (kTransposed) tma_load_2d(dst + C::kABytes, &tm_w, bar, (int)col0, (int)(kb * kBlock), pol);
+      mbar_expect_tx(bar, rows ? C::kABytes : C::kBBytes);
+      if (rows) tma_load_2d(dst, &tm_a, bar, (int)(kb * kBlock), (int)row0, pol);
+      else if (kTransposed) tma_load_2d(dst + C::kABytes, &tm_w, bar, (int)col0, (int)(kb * kBlock), pol);
       else tma_load_2d(dst + C::kABytes, &tm_w, bar, (int)(kb * kBlock), (int)col0, pol);
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if ((warp == 1 || warp == 3) && lane == 0) {
     const uint32_t idesc = make_idesc(kBN) | (kTransposed ? 1u << 16 : 0u);
-    for (uint32_t kb = kb0; kb < kb1; ++kb) {
-      const uint32_t it = kb - kb0, s = it % C::kStages, a = it % C::kAccStages;
-      if (!mbar_wait(smem_u32(&tempty_bar[a]), ((it / C::kAccStages) & 1) ^ 1, abort_flag) ||
-          !mbar_wait(smem_u32(&full_bar[s]), (it / C::kStages) & 1, abort_flag)) { g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break; }
+    for (uint32_t it = (uint32_t)warp >> 1; it < kb1 - kb0; it += 2) {
+      const uint32_t s = it % C::kStages, a = it % C::kAccStages;
+      if (!mbar_wait(smem_u32(&full_bar[s]), (it / C::kStages) & 1, abort_flag) ||
+          (it >= C::kAccStages && !mbar_wait(smem_u32(&tempty_bar[a]), ((it / C::kAccStages) & 1) ^ 1, abort_flag))) {
+        g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break;
+      }
       tc_fence_after();
       const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
       const uint64_t adesc = make_smem_desc(sa);
@@ -266,8 +278,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
 #pragma unroll
       for (int k = 0; k < kBlock / 32; ++k)
         umma_f8(tmem_base + a * kBN, adesc + 2 * k, bdesc + (kTransposed ? 256 : 2) * k, idesc, k > 0);
-      umma_commit(smem_u32(&empty_bar[s]));
-      umma_commit(smem_u32(&tfull_bar[a]));
+      umma_commit(smem_u32(&done_bar[s]));
     }
   } else if (warp >= 4) {
     constexpr int kCols = kBN / 2;                      // columns of this thread
@@ -299,7 +310,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
       for (int j = 0; j < 8; ++j) {
         if (!ok || base + j >= kb1) break;
         const uint32_t it = base + j - kb0, a = it % C::kAccStages;
-        if (!mbar_wait_warp(smem_u32(&tfull_bar[a]), (it / C::kAccStages) & 1, abort_flag)) {
+        if (!mbar_wait_warp(smem_u32(&done_bar[it % C::kStages]), (it / C::kStages) & 1, abort_flag)) {
           g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; ok = false; break;
         }
         tc_fence_after();
@@ -320,12 +331,15 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
       for (int j = 0; j < 8; ++j) s[j] = ahead[j];
     }
     __syncwarp();
-    // every MMA of this CTA has completed (the last accumulator stage was waited for), so the stages are free
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    float* dst = reinterpret_cast<float*>(smem) + (size_t)r * C::kOutPitch + wg * kCols;
+    if (ranks > 1) cluster_wait();
+    // row r belongs to the CTA of rank r / (128 / ranks)
+    const uint32_t share = 128u / ranks;
+    const uint32_t dst = map_to_rank(smem_u32(parts + ((size_t)(rank * share + r % share) * C::kOutPitch + wg * kCols)), r / share);
 #pragma unroll
-    for (int c = 0; c < kCols; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+    for (int c = 0; c < kCols; c += 4) st_cluster_f4(dst + 4 * c, acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
   }
+  __syncwarp();
+  if (warp < 4 && ranks > 1) cluster_wait();
 
   tc_fence_before();
   __syncthreads();
@@ -336,20 +350,21 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
   __syncwarp();
-  if (ranks > 1) cluster_barrier();
-  // rows r = rank, rank + ranks, ... ; a quarter, half or whole warp takes a row, a lane four neighbouring columns
-  constexpr uint32_t kLanes = kBN / 4, kRowsAtOnce = (kDnThreads / 32) * (32 / kLanes);
-  const uint32_t base = smem_u32(smem), c = (threadIdx.x % kLanes) * 4, col = col0 + c;
-#pragma unroll 2
-  for (uint32_t i = threadIdx.x / kLanes; i * ranks + rank < 128u; i += kRowsAtOnce) {
-    const uint32_t r = i * ranks + rank, row = row0 + r;
-    if (row >= g.m || col >= g.n) continue;
-    const uint32_t addr = base + (r * C::kOutPitch + c) * 4;
-    float4 sum = ld_cluster_f4(addr, 0);
+  if (ranks > 1) cluster_barrier();         // every part is in its owner's shared memory, and nothing reaches into a CTA after it
+  // a quarter, half or whole warp takes a row, a lane four neighbouring columns
+  constexpr uint32_t kLanes = kBN / 4, kRowsAtOnce = kDnThreads / kLanes;
+  const uint32_t share = 128u / ranks, first = row0 + rank * share, c = (threadIdx.x % kLanes) * 4, col = col0 + c;
+  if (first >= g.m || col >= g.n) return;
+  const uint32_t count = min(share, g.m - first);
+#pragma unroll 4
+  for (uint32_t r = threadIdx.x / kLanes; r < count; r += kRowsAtOnce) {
+    const float* p = parts + (size_t)r * C::kOutPitch + c;
+    float4 sum = *reinterpret_cast<const float4*>(p);
     for (uint32_t j = 1; j < ranks; ++j) {
-      const float4 p = ld_cluster_f4(addr, j);
-      sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+      const float4 q = *reinterpret_cast<const float4*>(p + (size_t)j * share * C::kOutPitch);
+      sum.x += q.x; sum.y += q.y; sum.z += q.z; sum.w += q.w;
     }
+    const uint32_t row = first + r;
     const uint64_t at = (uint64_t)row * g.out_pitch + col;
     if (g.out_vector && col + 4 <= g.n) {
       if (g.out_dtype == kDenseF32) {
@@ -372,8 +387,6 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
         if (col + j < g.n) dense_store(g.out, g.out_dtype, at + j, o[j]);
     }
   }
-  __syncwarp();
-  if (ranks > 1) cluster_barrier();            // nobody leaves while its partial tile is being read
 }
 
 }  // namespace netra

@@ -41,11 +41,6 @@ struct PairArgs {
   uint32_t m_tiles, n_tiles;              // of 256
 };
 
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
 // Arrival on a barrier of either CTA of the pair.  It hands over TMEM columns, whose reads tcgen05.wait::ld has completed and
 // tcgen05.fence orders; no other memory is handed over.
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t bar) {
