@@ -124,6 +124,12 @@ netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8
   }
 }
 
+__device__ __forceinline__ uint32_t pack_16bit(uint32_t dtype, float a, float b) {
+  if (dtype == kDenseF16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // ------------------------------------------------------------------------------------------
 // Product on the tensor cores.  A cluster owns 128 rows x kBN columns of the output and splits the K-blocks among
 // its CTAs; per K-block the raw sums leave TMEM and are promoted as acc = fma(part, sa * sw, acc), as in the grouped GEMMs.
@@ -158,7 +164,7 @@ struct DnArgs {
   uint64_t w_scale_col, w_scale_block;    // per 128 output columns, per K-block
   void* out;
   uint64_t out_pitch;
-  uint32_t out_dtype, out_vector;         // out_vector: four neighbouring elements are one aligned access
+  uint32_t out_dtype, out_vector;         // out_vector 1: four neighbouring elements are one aligned access; 2: rows start on 32-byte boundaries
   uint32_t m, n, k_blocks;                // rows, output columns, K-blocks
   uint32_t n_tiles;
 };
@@ -232,6 +238,8 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
   const uint32_t tile = blockIdx.x / ranks;
   const uint32_t row0 = (tile / g.n_tiles) * 128u, col0 = (tile % g.n_tiles) * (uint32_t)kBN;
+  // a whole tile of one CTA, its rows on 32-byte boundaries, goes straight from the registers to memory
+  const bool direct = ranks == 1 && g.out_vector == 2 && col0 + kBN <= g.n;
   const uint32_t kb0 = (uint32_t)((uint64_t)g.k_blocks * rank / ranks), kb1 = (uint32_t)((uint64_t)g.k_blocks * (rank + 1) / ranks);
 
   if (threadIdx.x == 0) {
@@ -330,13 +338,31 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] = ahead[j];
     }
-    __syncwarp();
-    if (ranks > 1) cluster_wait();
-    // row r belongs to the CTA of rank r / (128 / ranks)
-    const uint32_t share = 128u / ranks;
-    const uint32_t dst = map_to_rank(smem_u32(parts + ((size_t)(rank * share + r % share) * C::kOutPitch + wg * kCols)), r / share);
+    if (direct) {
+      if (row < g.m) {
+        const uint64_t at = (uint64_t)row * g.out_pitch + col0 + wg * kCols;
+        if (g.out_dtype == kDenseF32) {
 #pragma unroll
-    for (int c = 0; c < kCols; c += 4) st_cluster_f4(dst + 4 * c, acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+          for (int c = 0; c < kCols; c += 8) st_global_v8(reinterpret_cast<float*>(g.out) + at + c, acc + c);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 16) {
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = __uint_as_float(pack_16bit(g.out_dtype, acc[c + 2 * j], acc[c + 2 * j + 1]));
+            st_global_v8(reinterpret_cast<float*>(reinterpret_cast<uint16_t*>(g.out) + at + c), p);
+          }
+        }
+      }
+    } else {
+      __syncwarp();
+      if (ranks > 1) cluster_wait();
+      // row r belongs to the CTA of rank r / (128 / ranks)
+      const uint32_t share = 128u / ranks;
+      const uint32_t dst = map_to_rank(smem_u32(parts + ((size_t)(rank * share + r % share) * C::kOutPitch + wg * kCols)), r / share);
+#pragma unroll
+      for (int c = 0; c < kCols; c += 4) st_cluster_f4(dst + 4 * c, acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+    }
   }
   __syncwarp();
   if (warp < 4 && ranks > 1) cluster_wait();
@@ -349,42 +375,45 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
     tc_fence_after();
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
+  if (direct) return;
   __syncwarp();
   if (ranks > 1) cluster_barrier();         // every part is in its owner's shared memory, and nothing reaches into a CTA after it
-  // a quarter, half or whole warp takes a row, a lane four neighbouring columns
-  constexpr uint32_t kLanes = kBN / 4, kRowsAtOnce = kDnThreads / kLanes;
-  const uint32_t share = 128u / ranks, first = row0 + rank * share, c = (threadIdx.x % kLanes) * 4, col = col0 + c;
-  if (first >= g.m || col >= g.n) return;
+  const uint32_t share = 128u / ranks, first = row0 + rank * share;
+  if (first >= g.m) return;
   const uint32_t count = min(share, g.m - first);
-#pragma unroll 4
-  for (uint32_t r = threadIdx.x / kLanes; r < count; r += kRowsAtOnce) {
+  auto sum_at = [&](uint32_t r, uint32_t c, auto& to) {
+    using V = std::remove_reference_t<decltype(to)>;
     const float* p = parts + (size_t)r * C::kOutPitch + c;
-    float4 sum = *reinterpret_cast<const float4*>(p);
+    to = *reinterpret_cast<const V*>(p);
     for (uint32_t j = 1; j < ranks; ++j) {
-      const float4 q = *reinterpret_cast<const float4*>(p + (size_t)j * share * C::kOutPitch);
-      sum.x += q.x; sum.y += q.y; sum.z += q.z; sum.w += q.w;
+      const V q = *reinterpret_cast<const V*>(p + (size_t)j * share * C::kOutPitch);
+      if constexpr (sizeof(V) == 16) { to.x += q.x; to.y += q.y; to.z += q.z; to.w += q.w; }
+      else to += q;
     }
-    const uint32_t row = first + r;
-    const uint64_t at = (uint64_t)row * g.out_pitch + col;
-    if (g.out_vector && col + 4 <= g.n) {
-      if (g.out_dtype == kDenseF32) {
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at) = sum;
-      } else {
-        uint2 p;
-        if (g.out_dtype == kDenseF16) {
-          const __half2 lo = __floats2half2_rn(sum.x, sum.y), hi = __floats2half2_rn(sum.z, sum.w);
-          p = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        } else {
-          const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
-          p = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        }
-        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.out) + at) = p;
-      }
-    } else {
-      const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+  };
+  if (g.out_vector && col0 + kBN <= g.n) {
+    // a quarter, half or whole warp takes a row, a lane four neighbouring columns
+    constexpr uint32_t kLanes = kBN / 4, kRowsAtOnce = kDnThreads / kLanes;
+    const uint32_t c = (threadIdx.x % kLanes) * 4;
+#pragma unroll 4
+    for (uint32_t r = threadIdx.x / kLanes; r < count; r += kRowsAtOnce) {
+      float4 v;
+      sum_at(r, c, v);
+      const uint64_t at = (uint64_t)(first + r) * g.out_pitch + col0 + c;
+      if (g.out_dtype == kDenseF32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at) = v;
+      else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.out) + at) = make_uint2(pack_16bit(g.out_dtype, v.x, v.y), pack_16bit(g.out_dtype, v.z, v.w));
+    }
+  } else {
+    // rows on any boundary, or a tile that ends inside: neighbouring lanes store neighbouring elements
+    const uint32_t cols = min((uint32_t)kBN, g.n - col0);
+    for (uint32_t r = warp; r < count; r += kDnThreads / 32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < g.n) dense_store(g.out, g.out_dtype, at + j, o[j]);
+      for (uint32_t c = lane; c < (uint32_t)kBN; c += 32) {
+        if (c >= cols) continue;
+        float v;
+        sum_at(r, c, v);
+        dense_store(g.out, g.out_dtype, (uint64_t)(first + r) * g.out_pitch + col0 + c, v);
+      }
     }
   }
 }
@@ -614,7 +643,8 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   g.w_scale_col = transpose_w ? 1 : w_scale_pitch;
   g.w_scale_block = transpose_w ? w_scale_pitch : 1;
   g.out = out; g.out_pitch = out_pitch; g.out_dtype = out_dtype;
-  g.out_vector = (uintptr_t)out % (4 * dense_element_bytes(out_dtype)) == 0 && out_pitch % 4 == 0;
+  const uint64_t out_bytes = dense_element_bytes(out_dtype);
+  g.out_vector = ((uintptr_t)out | out_pitch * out_bytes) % 32 == 0 ? 2 : (uintptr_t)out % (4 * out_bytes) == 0 && out_pitch % 4 == 0 ? 1 : 0;
   g.m = m; g.n = n; g.k_blocks = (k + 127) / 128;
   const uint64_t m_tiles = (m + 127) / 128;
   const bool narrow = !transpose_w && m_tiles * ((n + 127) / 128) * 2 <= (uint64_t)sms;
