@@ -37,7 +37,7 @@ def binding_command() -> list[str]:
     includes = [*cpp_extension.include_paths(), "/usr/local/cuda/include", sysconfig.get_paths()["include"]]
     libs = cpp_extension.library_paths()
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", *[f"-I{i}" for i in includes], "-o", str(BINDING), str(HERE / "torch_binding.cpp"), *[f"-L{path}" for path in libs], f"-L{HERE}",
-            "-l:libnetra_sm100.so", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+            "-L/usr/local/cuda/lib64", "-l:libnetra_sm100.so", "-lcudart", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

@@ -568,7 +568,7 @@ int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, floa
   // four rows per lane once that still leaves every SM a few thousand lanes; below, one row each for the shortest chain
   const bool deep = (uint64_t)m * blocks >= 32768;
   const uint64_t grid = ((deep ? (m + 3) / 4 : m) * blocks + 15) / 16;
-  if (grid > 0x0fffffffull) return fail("dense_quantize_rows: too many blocks of 128 in one call");
+  if (grid > 0x00ffffffull) return fail("dense_quantize_rows: too many blocks of 128 in one call");
   const bool vector = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (x_pitch * dense_element_bytes(x_dtype)) % 16 == 0 &&
                       (uintptr_t)codes_fp8 % 8 == 0 && codes_pitch % 8 == 0;
   auto launch = [&](auto element, auto vec, auto rows) {
@@ -711,7 +711,9 @@ int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, 
 int netra_dense_status(uint32_t status_out[4]) {
   if (status_out == nullptr) return fail("dense_status: null pointer");
   cudaError_t e = cudaMemcpyFromSymbol(status_out, g_dense_status, 16);
-  return e == cudaSuccess ? 0 : fail_cuda("cudaMemcpyFromSymbol(dense status)", e);
+  const uint32_t clear[4] = {0, 0, 0, 0};
+  if (e == cudaSuccess && (status_out[0] | status_out[1] | status_out[2] | status_out[3])) e = cudaMemcpyToSymbol(g_dense_status, clear, 16);
+  return e == cudaSuccess ? 0 : fail_cuda("dense status", e);
 }
 
 }  // extern "C"

@@ -4,11 +4,13 @@
 // the host's share decides what a call costs: the same path through ctypes took 26 us per fp8_linear call and 130 us with its
 // gradient (Python autograd function).  Everything below the C ABI of include/netra_moe.h is unchanged; C callers need none of this.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -137,6 +139,19 @@ Tensor once_differentiable(Tensor grad, const Tensor& upstream) {
   return (*error)({grad.detach().requires_grad_()})[0];
 }
 
+// A leaf keeps its gradient node, with the stream it was made on, for as long as any graph of it lives.  If that was the default
+// stream, a backward pass captured on another one makes torch tie the two together, which CUDA forbids and which invalidates the
+// capture; so such a call is refused while the capture can still be ended.
+void check_capture(const Tensor& x) {
+  if (x.grad_fn()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
+  if (!node || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto made_on = node->stream();
+  TORCH_CHECK(!made_on.has_value() || made_on->id() != 0 || *made_on == c10::cuda::getCurrentCUDAStream(x.device().index()).unwrap(),
+              "an eager graph of this leaf, made on the default stream, is still alive: drop it (its loss and outputs) before capturing a "
+              "forward and backward pass of the same leaf, or capture with a fresh leaf");
+}
+
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& ws) {
     ctx->save_for_backward({w, ws});
@@ -152,7 +167,10 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const Tensor& ws) {
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor");
   TORCH_CHECK_VALUE(x.dim() > 0 && w.dim() == 2 && x.size(-1) == w.size(1), "x must have as many columns as the weight");
   check_weight(w, ws, x.device());
-  if (x.requires_grad() && at::GradMode::is_enabled()) return LinearFunction::apply(x, w, ws);
+  if (x.requires_grad() && at::GradMode::is_enabled()) {
+    check_capture(x);
+    return LinearFunction::apply(x, w, ws);
+  }
   return linear(x, w, ws, false);
 }
 
@@ -229,7 +247,10 @@ Tensor balance_loss(const Tensor& logits, const Tensor& counts, const std::optio
   TORCH_CHECK_VALUE(counts.scalar_type() == at::kInt && counts.device() == logits.device() && counts.dim() == 1 && counts.size(0) == experts &&
                         counts.is_contiguous(), "counts must be a contiguous int32 [experts] tensor on the same device");
   const uint8_t* mask = mask_of(token_mask, tokens, logits.device());
-  if (logits.requires_grad() && at::GradMode::is_enabled()) return BalanceFunction::apply(logits, counts, token_mask);
+  if (logits.requires_grad() && at::GradMode::is_enabled()) {
+    check_capture(logits);
+    return BalanceFunction::apply(logits, counts, token_mask);
+  }
   return std::get<0>(balance_forward(as_rows(logits, "logits"), counts, mask));
 }
 

@@ -280,6 +280,61 @@ def test_streams_and_captured_graphs():
     dense.check_status()
 
 
+def test_capture_beside_a_living_eager_graph_of_the_leaf_is_refused():
+    """torch itself cannot capture this backward pass; the call says so while the capture can still be ended."""
+    w, ws = make_weight(64, 128, 1)
+    leaf = torch.randn(4, 128, device="cuda").requires_grad_()
+    alive = dense.fp8_linear(leaf, w, ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            dense.fp8_linear(leaf, w, ws)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            balance.balance_loss(leaf, torch.ones(128, dtype=torch.int32, device="cuda"))
+        plain = dense.fp8_linear(leaf.detach(), w, ws)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, alive.detach())
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, second = dense.fp8_linear(leaf, w, ws), dense.fp8_linear(leaf, w, ws)
+        (dx,) = torch.autograd.grad(first.sum() + second.sum(), leaf)
+    graph.replay()
+    torch.cuda.synchronize()
+    (want,) = torch.autograd.grad(dense.fp8_linear(leaf, w, ws).sum() * 2, leaf)
+    assert torch.allclose(dx, want, rtol=2.0 ** -22, atol=0)
+
+
+def test_second_derivatives_are_refused():
+    w, ws = make_weight(32, 128, 1)
+    x = torch.randn(3, 128, device="cuda").requires_grad_()
+    dy = torch.ones(3, 32, device="cuda").requires_grad_()
+    (dx,) = torch.autograd.grad(dense.fp8_linear(x, w, ws), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        dx.sum().backward()
+    counts = torch.ones(128, dtype=torch.int32, device="cuda")
+    (dz,) = torch.autograd.grad(balance.balance_loss(x, counts), x, torch.ones((), device="cuda").requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        dz.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 activations and outputs: sampled rows against the same rows alone (whole rows are quantised and multiplied
+    independently of their neighbours, through the same kernel only if the sizes say so: FP32 rounding apart, as derived above)."""
+    m, n, k = 70001, 32784, 144
+    w, ws = make_weight(n, k, 9)
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(2))
+    y = dense.fp8_linear(x, w, ws)
+    pick = torch.tensor([0, 1, 32767, 65535, 65536, 65537, 69999, 70000])
+    check_product(y[pick.cuda()], *quantize_definition(x[pick.cuda()]), w, ws)
+    codes, scale = dense.quantize_rows(y)                             # 2.3e9 elements
+    want, want_scale = quantize_definition(y[pick.cuda()])
+    assert torch.equal(scale[pick.cuda()].cpu(), want_scale)
+    assert torch.equal(codes.view(torch.uint8)[pick.cuda()].cpu(), want.view(torch.uint8))
+    dense.check_status()
+
+
 def test_refusals():
     x = torch.zeros(4, 256, device="cuda")
     w, ws = make_weight(64, 256, 1)
