@@ -17,6 +17,7 @@ extern "C" __global__ void __launch_bounds__(256)
 netra_expert_counts_sm100(const void* __restrict__ ids, uint32_t wide, uint64_t id_pitch, const uint8_t* __restrict__ mask,
                           int32_t* __restrict__ counts, uint64_t tokens, uint32_t slots, uint32_t experts) {
   __shared__ int hist[kBalMaxExperts];
+  begin_grid();
   for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
   const uint32_t pairs = (uint32_t)tokens * slots, step = gridDim.x * 256u;       // the host keeps pairs below 2^31
@@ -150,6 +151,7 @@ netra_balance_loss_sm100(const T* __restrict__ z, uint64_t pitch, const int32_t*
   __shared__ double warp_part[kBalThreads / 32];
   __shared__ unsigned long long warp_rows[kBalThreads / 32];
   __shared__ bool last;
+  begin_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double sum = 0.0;
   unsigned long long rows = 0;
@@ -196,6 +198,7 @@ netra_balance_loss_grad_sm100(T* __restrict__ grad, uint64_t grad_pitch, const T
                               const int32_t* __restrict__ counts, const uint8_t* __restrict__ mask, const float* __restrict__ scale,
                               const float* __restrict__ upstream, uint64_t tokens, uint32_t experts) {
   using L = BalLane<T, kAligned, kPer>;
+  begin_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float c[kPer], v[kPer], inv;
   const float per_count = L::counts(c, counts, experts, lane);
@@ -276,9 +279,9 @@ int netra_expert_counts_launch(int32_t* counts_i32, const void* ids, uint32_t id
   const uint64_t pairs = tokens * slots;
   if (pairs == 0) return 0;
   const uint64_t blocks = (pairs + 511) / 512;
-  netra_expert_counts_sm100<<<(unsigned)(blocks < 296 ? blocks : 296), 256, 0, stream>>>(ids, id_bytes == 8, id_pitch, token_mask, counts_i32,
-                                                                                        tokens, slots, experts);
-  return check_launch("expert_counts launch");
+  return launched("expert_counts launch",
+                  launch_dependent(netra_expert_counts_sm100, dim3((unsigned)(blocks < 296 ? blocks : 296)), 256, 0, stream, 1, ids, (uint32_t)(id_bytes == 8),
+                                   id_pitch, token_mask, counts_i32, tokens, slots, experts));
 }
 
 uint64_t netra_balance_loss_workspace_bytes(void) { return 16 + kBalMaxBlocks * sizeof(BalPartial); }
@@ -294,12 +297,13 @@ int netra_balance_loss_launch(float* loss_f32, float* scale_f32, const void* log
   cudaError_t e = cudaMemsetAsync(ticket, 0, sizeof(uint32_t), stream);
   if (e != cudaSuccess) return fail_cuda("balance_loss memset", e);
   const uint32_t grid = balance_blocks(tokens);
+  cudaError_t launch = cudaSuccess;
   balance_shape(dtype, balance_aligned(logits, pitch, dtype, experts), experts, [&](auto element, auto access, auto per) {
     using T = decltype(element);
-    netra_balance_loss_sm100<T, decltype(access)::value, decltype(per)::value><<<grid, kBalThreads, 0, stream>>>(
-        (const T*)logits, pitch, counts_i32, token_mask, loss_f32, scale_f32, partial, ticket, tokens, experts);
+    launch = launch_dependent(netra_balance_loss_sm100<T, decltype(access)::value, decltype(per)::value>, dim3(grid), kBalThreads, 0, stream, 1,
+                              (const T*)logits, pitch, counts_i32, token_mask, loss_f32, scale_f32, partial, ticket, tokens, experts);
   });
-  return check_launch("balance_loss launch");
+  return launched("balance_loss launch", launch);
 }
 
 int netra_balance_loss_grad_launch(void* grad, uint64_t grad_pitch, const void* logits, uint32_t dtype, uint64_t pitch, const int32_t* counts_i32,
@@ -311,12 +315,13 @@ int netra_balance_loss_grad_launch(void* grad, uint64_t grad_pitch, const void* 
   if ((uintptr_t)grad % dense_element_bytes(dtype)) return fail("balance_loss_grad: the gradient is not aligned to its element");
   const uint32_t grid = balance_blocks(tokens);
   const bool aligned = balance_aligned(logits, pitch, dtype, experts) && balance_aligned(grad, grad_pitch, dtype, experts);
+  cudaError_t launch = cudaSuccess;
   balance_shape(dtype, aligned, experts, [&](auto element, auto access, auto per) {
     using T = decltype(element);
-    netra_balance_loss_grad_sm100<T, decltype(access)::value, decltype(per)::value><<<grid, kBalThreads, 0, stream>>>(
-        (T*)grad, grad_pitch, (const T*)logits, pitch, counts_i32, token_mask, scale_f32, upstream_f32, tokens, experts);
+    launch = launch_dependent(netra_balance_loss_grad_sm100<T, decltype(access)::value, decltype(per)::value>, dim3(grid), kBalThreads, 0, stream, 1,
+                              (T*)grad, grad_pitch, (const T*)logits, pitch, counts_i32, token_mask, scale_f32, upstream_f32, tokens, experts);
   });
-  return check_launch("balance_loss_grad launch");
+  return launched("balance_loss_grad launch", launch);
 }
 
 }  // extern "C"

@@ -87,7 +87,7 @@ netra_dense_fp8_few_sm100(const FewArgs g) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int grp = lane >> 2, t = lane & 3;
   const uint32_t n0 = blockIdx.x * kFewRows, blocks = (g.k + kBlock - 1) / kBlock;
-  grid_dependency_wait();
+  begin_grid();
   const uint8_t* w_lo = g.w + (uint64_t)min(n0 + grp, g.n - 1) * g.w_pitch;        // rows past the end: computed, not stored
   const uint8_t* w_hi = g.w + (uint64_t)min(n0 + grp + 8, g.n - 1) * g.w_pitch;
   const float* ws = g.w_scale + (uint64_t)(n0 / kBlock) * g.w_scale_pitch;

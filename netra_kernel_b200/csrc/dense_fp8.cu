@@ -27,10 +27,14 @@ __device__ __forceinline__ void dense_store(void* p, uint32_t dtype, size_t i, f
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
-// The product may be launched while the kernel before it is still running (programmatic dependent launch): the set-up of its
-// barriers and TMEM overlaps that kernel's end, and every access to global memory comes after the wait.
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_dependency_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The kernels here are launched while the kernel before them on the stream may still be running (programmatic dependent
+// launch): their launch, and the set-up of barriers and TMEM, overlap its end.  Every access to global memory comes after
+// begin_grid(), which waits until that kernel has completed and its writes are visible - stream order, as for any launch - and
+// lets the next such launch come as early.
+__device__ __forceinline__ void begin_grid() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 // ------------------------------------------------------------------------------------------
 // Row quantiser.  Sixteen lanes own one block of 128 columns of kRows neighbouring rows, eight neighbouring columns each: a
@@ -69,7 +73,7 @@ template <typename T, bool kVector, int kRows>
 __global__ void __launch_bounds__(256)
 netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8_t* __restrict__ codes, uint64_t codes_pitch,
                                 float* __restrict__ scale, uint64_t scale_row, uint64_t scale_block, uint32_t m, uint32_t k) {
-  grid_dependency_trigger();
+  begin_grid();
   const uint32_t blocks = (k + kBlock - 1) / kBlock;
   const uint32_t item = (blockIdx.x * 256u + threadIdx.x) >> 4;
   const uint32_t group = item / blocks, b = item - group * blocks;
@@ -255,7 +259,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   if (ranks > 1) cluster_arrive();          // this CTA is running: others may store into its shared memory
-  grid_dependency_wait();                   // nothing above touches global memory
+  begin_grid();                             // nothing above touches global memory
 
   if ((warp == 0 || warp == 2) && lane == 0) {
     const uint64_t pol = policy_evict_last();
@@ -425,6 +429,21 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
 
 namespace {
 
+// Launch as a programmatic dependent of the kernel before it (the kernel calls begin_grid); cluster = 1: no cluster.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, uint32_t block, size_t smem, cudaStream_t stream, uint32_t cluster, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid; cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+int launched(const char* what, cudaError_t e) { return e == cudaSuccess ? check_launch(what) : fail_cuda(what, e); }
+
 uint64_t dense_element_bytes(uint32_t dtype) { return dtype == kDenseF32 ? 4 : 2; }
 
 // Byte tensor of `rows` rows of `cols` codes, `pitch` bytes apart; box 128 bytes x box_rows, 128-byte swizzle.
@@ -511,22 +530,17 @@ constexpr uint32_t kFewMaxRows = 16, kFewMaxCodeRows = 32;
 int launch_few(const FewArgs& g, uint32_t source, cudaStream_t stream) {
   const uint32_t blocks = (g.k + 127) / 128, warps = blocks < 2 ? 1 : blocks / 2 < 16 ? (blocks + 1) / 2 : 16;
   const uint32_t tiles = g.m <= 8 ? 1 : g.m <= 16 ? 2 : 4;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((g.n + kFewRows - 1) / kFewRows); cfg.blockDim = dim3(32 * warps);
-  cfg.dynamicSmemBytes = warps * tiles * 8 * kFewRows * sizeof(float);
-  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
+  const dim3 grid((g.n + kFewRows - 1) / kFewRows);
+  const size_t smem = warps * tiles * 8 * kFewRows * sizeof(float);
   auto launch = [&](auto element) {
     using T = decltype(element);
     if constexpr (sizeof(T) == 1) {
-      if (tiles == 4) return cudaLaunchKernelEx(&cfg, netra_dense_fp8_few_sm100<T, 4>, g);
+      if (tiles == 4) return launch_dependent(netra_dense_fp8_few_sm100<T, 4>, grid, 32 * warps, smem, stream, 1, g);
     }
-    return tiles == 1 ? cudaLaunchKernelEx(&cfg, netra_dense_fp8_few_sm100<T, 1>, g) : cudaLaunchKernelEx(&cfg, netra_dense_fp8_few_sm100<T, 2>, g);
+    return launch_dependent(tiles == 1 ? netra_dense_fp8_few_sm100<T, 1> : netra_dense_fp8_few_sm100<T, 2>, grid, 32 * warps, smem, stream, 1, g);
   };
   const cudaError_t e = source == 3 ? launch((uint8_t)0) : source == kDenseF32 ? launch(0.0f) : source == kDenseF16 ? launch(__half{}) : launch(__nv_bfloat16{});
-  return e == cudaSuccess ? check_launch("dense_fp8 launch (few rows)") : fail_cuda("dense_fp8 launch (few rows)", e);
+  return launched("dense_fp8 launch (few rows)", e);
 }
 
 
@@ -573,18 +587,16 @@ int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, floa
                       (uintptr_t)codes_fp8 % 8 == 0 && codes_pitch % 8 == 0;
   auto launch = [&](auto element, auto vec, auto rows) {
     using T = decltype(element);
-    netra_dense_quantize_rows_sm100<T, decltype(vec)::value, decltype(rows)::value><<<(unsigned)grid, 256, 0, stream>>>(
-        (const T*)x, x_pitch, (uint8_t*)codes_fp8, codes_pitch, scale_f32, scale_row_stride, scale_block_stride, m, k);
+    return launch_dependent(netra_dense_quantize_rows_sm100<T, decltype(vec)::value, decltype(rows)::value>, dim3((unsigned)grid), 256, 0, stream, 1,
+                            (const T*)x, x_pitch, (uint8_t*)codes_fp8, codes_pitch, scale_f32, scale_row_stride, scale_block_stride, m, k);
   };
   auto shape = [&](auto element) {
-    if (!vector) { if (deep) launch(element, std::false_type{}, std::integral_constant<int, 4>{}); else launch(element, std::false_type{}, std::integral_constant<int, 1>{}); }
-    else if (deep) launch(element, std::true_type{}, std::integral_constant<int, 4>{});
-    else launch(element, std::true_type{}, std::integral_constant<int, 1>{});
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 1> one;
+    if (vector) return deep ? launch(element, std::true_type{}, four) : launch(element, std::true_type{}, one);
+    return deep ? launch(element, std::false_type{}, four) : launch(element, std::false_type{}, one);
   };
-  if (x_dtype == kDenseBf16) shape(__nv_bfloat16{});
-  else if (x_dtype == kDenseF16) shape(__half{});
-  else shape(0.0f);
-  return check_launch("dense_quantize_rows launch");
+  return launched("dense_quantize_rows launch", x_dtype == kDenseBf16 ? shape(__nv_bfloat16{}) : x_dtype == kDenseF16 ? shape(__half{}) : shape(0.0f));
 }
 
 int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pitch, const void* a_fp8, uint64_t a_pitch,
@@ -623,19 +635,13 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
     if (p.tma_store)
       if (int rc = encode_output(&tm_out, out, m, n, out_pitch, size)) return rc;
     const uint64_t pairs = m256 * n256 < (uint64_t)(sms / 2) ? m256 * n256 : (uint64_t)(sms / 2);
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = PairCfg::kSmemBytes;
-    cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 1;
     auto launch = [&](auto element) {
       using T = decltype(element);
-      return transpose_w ? cudaLaunchKernelEx(&cfg, netra_dense_fp8_pair_sm100<true, T>, tm_a, tm_w, tm_out, p)
-                         : cudaLaunchKernelEx(&cfg, netra_dense_fp8_pair_sm100<false, T>, tm_a, tm_w, tm_out, p);
+      return launch_dependent(transpose_w ? netra_dense_fp8_pair_sm100<true, T> : netra_dense_fp8_pair_sm100<false, T>, dim3((unsigned)(2 * pairs)),
+                              kPairThreads, PairCfg::kSmemBytes, stream, 1, tm_a, tm_w, tm_out, p);
     };
     const cudaError_t e = out_dtype == kDenseF32 ? launch(0.0f) : out_dtype == kDenseF16 ? launch(__half{}) : launch(__nv_bfloat16{});
-    return e == cudaSuccess ? check_launch("dense_fp8_matmul launch") : fail_cuda("dense_fp8_matmul launch", e);
+    return launched("dense_fp8_matmul launch", e);
   }
   DnArgs g;
   g.a_scale = a_scale_f32; g.a_scale_row = a_scale_row_stride; g.a_scale_block = a_scale_block_stride;
@@ -655,27 +661,12 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   while (split < 8 && tiles * split * 2 <= (uint64_t)sms && g.k_blocks >= split * 4) split *= 2;
   if (tiles * split > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
   if (int rc = encode_codes(&tm_w, w_fp8, w_rows, w_cols, w_pitch, transpose_w ? 128 : bn)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(tiles * split)); cfg.blockDim = dim3(kDnThreads);
-  cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = 2;
-  cudaError_t e;
-  if (transpose_w) {
-    cfg.dynamicSmemBytes = DnCfg<128>::kSmemBytes;
-    e = cudaLaunchKernelEx(&cfg, netra_dense_fp8_matmul_sm100<128, true>, tm_a, tm_w, g);
-  } else if (narrow) {
-    cfg.dynamicSmemBytes = DnCfg<64>::kSmemBytes;
-    e = cudaLaunchKernelEx(&cfg, netra_dense_fp8_matmul_sm100<64, false>, tm_a, tm_w, g);
-  } else {
-    cfg.dynamicSmemBytes = DnCfg<128>::kSmemBytes;
-    e = cudaLaunchKernelEx(&cfg, netra_dense_fp8_matmul_sm100<128, false>, tm_a, tm_w, g);
-  }
-  if (e != cudaSuccess) return fail_cuda("dense_fp8_matmul launch", e);
-  return check_launch("dense_fp8_matmul launch");
+  const dim3 grid((unsigned)(tiles * split));
+  const cudaError_t e =
+      transpose_w ? launch_dependent(netra_dense_fp8_matmul_sm100<128, true>, grid, kDnThreads, DnCfg<128>::kSmemBytes, stream, split, tm_a, tm_w, g)
+      : narrow    ? launch_dependent(netra_dense_fp8_matmul_sm100<64, false>, grid, kDnThreads, DnCfg<64>::kSmemBytes, stream, split, tm_a, tm_w, g)
+                  : launch_dependent(netra_dense_fp8_matmul_sm100<128, false>, grid, kDnThreads, DnCfg<128>::kSmemBytes, stream, split, tm_a, tm_w, g);
+  return launched("dense_fp8_matmul launch", e);
 }
 
 // codes [m, k rounded up to 16] and, behind them, scales [ceil(k/128)][m]

@@ -128,7 +128,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   cluster_barrier();                                  // the peer's barriers exist before anything reports to them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  grid_dependency_wait();                             // nothing above touches global memory
+  begin_grid();                                       // nothing above touches global memory
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairRegsLow));
