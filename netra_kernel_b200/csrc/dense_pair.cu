@@ -3,13 +3,19 @@
 // Every K-block of 128 leaves 256 x 256 raw sums in TMEM which the CUDA cores scale by sa[row] * sw[tile] and add up in
 // registers, so three things have to overlap: the tensor core (512 cycles a K-block), the operands (32 KB per CTA and
 // K-block: a pair fetches its weight tile once, half each; one CTA alone would need 48 KB, more than the L2 delivers in that
-// time) and the promotion (128 KB read out of TMEM and 32,768 multiply-adds per CTA).  Sixteen promotion warps, four per
-// scheduler, hide the latencies of that chain that eight cannot; a thread keeps 64 columns of its row.
+// time) and the promotion (128 KB read out of TMEM and 32,768 multiply-adds per CTA).  What bounds it is the chain MMA ->
+// commit -> promotion -> release -> MMA on one accumulator stage: 930 cycles per K-block at two stages, of which the commit
+// across two CTAs alone takes about 400.  Hence:
+//   * sixteen promotion warps, four per scheduler, hide latencies that eight cannot; a thread keeps 64 columns of its row;
+//   * a K-block is multiplied and handed over in two halves of 128 columns, each with its own barriers (140 -> 133 us at
+//     16384 x 4096 x 2048), by two issuing threads that take alternate K-blocks (151 -> 137 us);
+//   * the scales go through shared memory, four K-blocks ahead: loaded by the promotion warps themselves, one K-block ahead,
+//     they were what the loop waited for (172 -> 151 us).
+// 16384 x 4096 x 2048: 133 us = 2.06 PFLOP/s in a burst, 157 us back to back for seconds (1,000 W cap, 1.59 GHz).
+//
 //   warp 0: TMA producer (each CTA its own 128 rows and its own 128 weight rows; both report to the leader's barrier)
-//   warps 1 and 3: MMA issuers (leader CTA) or the relay of the peer's releases (warp 1, which also owns TMEM), warp 2: scales,
+//   warps 1 and 3: MMA issuers (leader CTA) or relays of the peer's releases (warp 1 also owns TMEM), warp 2: scales,
 //   warps 4..19: promotion and store
-// The scales go through shared memory, four K-blocks ahead: loaded by the promotion warps themselves, one K-block ahead, they
-// were what the loop waited for (785 ns a K-block against 600 with the loads dropped).
 // The grid is persistent; the accumulators are double-buffered in TMEM, so the next item's first two K-blocks run while an
 // item is being stored.  Every wait is bounded; on expiry the CTA records a code and drains.
 namespace netra {
@@ -27,6 +33,9 @@ struct PairCfg {
   static constexpr int kScaleSlotFloats = 128 + 4;                // 128 rows, two weight tiles
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kScaleSlots * kScaleSlotFloats * 4 + 256;
   static_assert(kSmemBytes <= 232448, "exceeds the shared memory of one SM");
+  // the barriers of the two accumulator stages are 16 bytes apart and told apart by that address bit
+  static constexpr int kTemptyOffset = kStages * kStageBytes + kStagingBytes + kScaleSlots * kScaleSlotFloats * 4 + 3 * kStages * 8;
+  static_assert(kTemptyOffset % 32 == 0, "the release barriers' address bit");
 };
 
 struct PairArgs {
@@ -103,9 +112,9 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   uint8_t* staging = smem + C::kStages * C::kStageBytes;
   float* scales = reinterpret_cast<float*>(staging + C::kStagingBytes);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kScaleSlots * C::kScaleSlotFloats);
-  uint64_t* done_bar = full_bar + C::kStages;         // a stage's MMAs are done and its scales are there
-  uint64_t* tempty_bar = done_bar + C::kStages;       // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  uint64_t* done_bar = full_bar + C::kStages;         // [stage][half]: the MMAs of a stage's half are done and its scales are there
+  uint64_t* tempty_bar = done_bar + 2 * C::kStages;   // [accumulator stage][half]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 4);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -113,8 +122,8 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   const uint32_t items = g.m_tiles * g.n_tiles, pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&done_bar[s]), 2); }
-    for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&tempty_bar[a]), rank == 0 ? 17 : 16);   // promotion warps, and the peer's relay
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&done_bar[2 * s]), 2); mbar_init(smem_u32(&done_bar[2 * s + 1]), 2); }
+    for (int a = 0; a < 4; ++a) mbar_init(smem_u32(&tempty_bar[a]), rank == 0 ? 9 : 8);     // promotion warps, and the peer's relay
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -142,7 +151,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
         const int row = (int)(mt * 256 + rank * 128), col = (int)(nt * 256 + rank * 128);
         for (uint32_t kb = 0; kb < g.k_blocks; ++kb, ++it) {
           const uint32_t s = it % C::kStages;
-          if (!mbar_wait(smem_u32(&done_bar[s]), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
+          if (!mbar_wait(smem_u32(&done_bar[2 * s + 1]), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
             g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; ok = false; break;
           }
           if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * C::kStageBytes);
@@ -155,33 +164,39 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
     } else if ((warp == 1 || warp == 3) && lane == 0 && rank == 0) {
       // Two threads take alternate K-blocks, each its own accumulator stage: while one feeds its four MMAs to the tensor pipe,
       // the other is already through its waits.  The operands, which are early, are waited for first.
-      const uint32_t idesc = (1u << 4) | (kTransposed ? 1u << 16 : 0u) | ((256u >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (kTransposed ? 1u << 16 : 0u) | ((128u >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
       const uint32_t a = (uint32_t)warp >> 1, mine = pair < items ? (items - 1 - pair) / pairs + 1 : 0;
       const uint64_t total = (uint64_t)mine * g.k_blocks;
       uint32_t phase = 1;
-      for (uint64_t it = a; it < total; it += 2, phase ^= 1) {
+      bool ok = true;
+      for (uint64_t it = a; ok && it < total; it += 2, phase ^= 1) {
         const uint32_t s = (uint32_t)it % C::kStages;
-        if (!mbar_wait(smem_u32(&full_bar[s]), (uint32_t)(it / C::kStages) & 1, abort_flag) ||
-            !mbar_wait(smem_u32(&tempty_bar[a]), phase, abort_flag)) {
-          g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break;
-        }
-        tc_fence_after();
+        ok = mbar_wait(smem_u32(&full_bar[s]), (uint32_t)(it / C::kStages) & 1, abort_flag);
         const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
         const uint64_t adesc = make_smem_desc(sa);
         const uint64_t bdesc = kTransposed ? make_smem_desc_mn(sa + 128 * kBlock) : make_smem_desc(sa + 128 * kBlock);
 #pragma unroll
-        for (int k = 0; k < kBlock / 32; ++k)
-          umma_f8_pair(tmem_base + a * 256, adesc + 2 * k, bdesc + (kTransposed ? 256 : 2) * k, idesc, k > 0);
-        umma_commit_pair(smem_u32(&done_bar[s]));
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && mbar_wait(smem_u32(&tempty_bar[2 * a + h]), phase, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          // half h: 64 weight rows (or columns) of either CTA
+          const uint64_t bhalf = bdesc + (kTransposed ? 64 >> 4 : 64 * kBlock >> 4) * h;
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k)
+            umma_f8_pair(tmem_base + a * 256 + h * 128, adesc + 2 * k, bhalf + (kTransposed ? 256 : 2) * k, idesc, k > 0);
+          umma_commit_pair(smem_u32(&done_bar[2 * s + h]));
+        }
       }
-    } else if (warp == 1 && lane == 0) {
-      // The peer's sixteen releases reach the leader as one arrival.
-      const uint32_t mine = pair < items ? (items - 1 - pair) / pairs + 1 : 0;
+      if (!ok) { g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; }
+    } else if ((warp == 1 || warp == 3) && lane == 0) {
+      // The peer's eight releases of a half reach the leader as one arrival.
+      const uint32_t h = (uint32_t)warp >> 1, mine = pair < items ? (items - 1 - pair) / pairs + 1 : 0;
       const uint64_t total = (uint64_t)mine * g.k_blocks;
       for (uint64_t it = 0; it < total; ++it) {
-        const uint32_t a = (uint32_t)it & 1;
-        if (!mbar_wait(smem_u32(&tempty_bar[a]), (uint32_t)(it >> 1) & 1, abort_flag)) { g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break; }
-        mbar_arrive_peer(map_to_rank(smem_u32(&tempty_bar[a]), 0));
+        const uint32_t bar = smem_u32(&tempty_bar[2 * ((uint32_t)it & 1) + h]);
+        if (!mbar_wait(bar, (uint32_t)(it >> 1) & 1, abort_flag)) { g_dense_status[0] = kStatusMmaTimeout; *abort_flag = 1; break; }
+        mbar_arrive_peer(map_to_rank(bar, 0));
       }
     } else if (warp == 2) {
       // An accumulator stage counts as full when its MMAs are done and its K-block's scales are in their slot.  Once K-block
@@ -210,13 +225,13 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
       };
       for (int j = 0; j < 4; ++j) load();
       for (uint64_t it = 0; it < total; ++it) {
-        if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&done_bar[(it - 2) % C::kStages]), (uint32_t)((it - 2) / C::kStages) & 1, abort_flag))) {
+        if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&done_bar[2 * ((it - 2) % C::kStages) + 1]), (uint32_t)((it - 2) / C::kStages) & 1, abort_flag))) {
           g_dense_status[0] = kStatusProducerTimeout; *abort_flag = 1; break;
         }
         load();
         asm volatile("cp.async.wait_group 4;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&done_bar[it % C::kStages]));
+        if (lane < 2) mbar_arrive(smem_u32(&done_bar[2 * (it % C::kStages) + lane]));
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
@@ -227,23 +242,23 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
     // This loop is paced by the instructions its sixteen warps issue (four per scheduler), so what can be carried from one
     // K-block to the next is carried: the barrier's address and phase, the scales' slot (four stages and two phases make the
     // eight slots), the TMEM column of the accumulator stage.
-    const uint32_t bar0 = smem_u32(&done_bar[0]);
-    const uint32_t slot0 = smem_u32(scales) + (uint32_t)(quad * 32 + lane) * 4u, tile_scale = (uint32_t)(128 + (wg >> 1) - (quad * 32 + lane)) * 4u;
+    const uint32_t bar0 = smem_u32(&done_bar[wg >> 1]);
+    const uint32_t slot0 = smem_u32(scales) + (uint32_t)(quad * 32 + lane) * 4u, tile_scale = (uint32_t)(128 + (wg & 1) - (quad * 32 + lane)) * 4u;
     uint32_t stage = 0, phase = 0, column = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(wg * 64);
     static_assert(C::kScaleSlots == 2 * C::kStages, "a slot is a stage and the parity of its phase");
     const bool first_lane = lane == 0;
-    uint32_t release = smem_u32(&tempty_bar[0]);
+    uint32_t release = smem_u32(&tempty_bar[wg >> 1]);
     bool ok = true;
     for (uint32_t item = pair; ok && item < items; item += pairs) {
       uint32_t mt, nt;
       pair_item(item, g.m_tiles, g.n_tiles, mt, nt);
-      const uint32_t row0 = mt * 256 + rank * 128 + quad * 32, col0 = nt * 256 + wg * 64;
+      const uint32_t row0 = mt * 256 + rank * 128 + quad * 32, col0 = nt * 256 + (wg & 1) * 128 + (wg >> 1) * 64;
       float2 acc[32];
 #pragma unroll
       for (int c = 0; c < 32; ++c) acc[c] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
       for (uint32_t kb = 0; kb < g.k_blocks; ++kb) {
-        const uint32_t bar = bar0 + 8 * stage;
+        const uint32_t bar = bar0 + 16 * stage;
         if (!mbar_wait_warp(bar, phase, abort_flag)) { ok = false; break; }
         tc_fence_after();
         uint32_t v[32];
@@ -260,7 +275,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
         tc_fence_before();
         __syncwarp();
         if (first_lane) mbar_arrive(release);
-        release ^= 8;
+        release ^= 16;
         column ^= 256;
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[16 + c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), s2, acc[16 + c]);
