@@ -449,8 +449,8 @@ int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, floa
                                      uint64_t scale_block_stride, const void* x, uint32_t x_dtype, uint64_t x_pitch,
                                      uint32_t m, uint32_t k, cudaStream_t stream);
 
-/* out[m, n] = sum over K-blocks b of a_scale[m,b] * w_scale[.,.] * sum_{k in b} a[m,k] * w, FP32, blocks ascending, one
- * rounding to out_dtype.  transpose_w = 0: w is [n, k] (a linear layer's weight); 1: w is [k, n] as stored (the gradient to
+/* out[m, n] = sum over K-blocks b of a_scale[m,b] * w_scale[.,.] * sum_{k in b} a[m,k] * w in FP32, one rounding to
+ * out_dtype.  The order of the sum depends on the sizes only, so calls repeat bit for bit.  transpose_w = 0: w is [n, k] (a linear layer's weight); 1: w is [k, n] as stored (the gradient to
  * a linear layer's input: w_rows is the reduction).  Scale strides as above. */
 int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pitch, const void* a_fp8, uint64_t a_pitch,
                                   const float* a_scale_f32, uint64_t a_scale_row_stride, uint64_t a_scale_block_stride,

@@ -527,8 +527,11 @@ constexpr uint32_t kDenseMaxSize = 1u << 26;
 constexpr uint32_t kFewMaxRows = 16, kFewMaxCodeRows = 32;
 
 // Product of few rows; x of type code `source` (kDense*, or 3 for codes with their scales).
-int launch_few(const FewArgs& g, uint32_t source, cudaStream_t stream) {
-  const uint32_t blocks = (g.k + 127) / 128, warps = blocks < 2 ? 1 : blocks / 2 < 16 ? (blocks + 1) / 2 : 16;
+int launch_few(const FewArgs& g, uint32_t source, int sms, cudaStream_t stream) {
+  // two K-blocks a warp at first; sixteen warps, or eight where two CTAs an SM overlap their starts and ends (1 x 8192 x 8192:
+  // 17.9 us with sixteen, 16.0 us with eight; 1 x 4096 x 4096: 5.8 us against 6.1 us)
+  const uint32_t blocks = (g.k + 127) / 128, most = (g.n + kFewRows - 1) / kFewRows > 2u * (uint32_t)sms ? 8 : 16;
+  const uint32_t warps = (blocks + 1) / 2 < most ? (blocks + 1) / 2 : most;
   const uint32_t tiles = g.m <= 8 ? 1 : g.m <= 16 ? 2 : 4;
   const dim3 grid((g.n + kFewRows - 1) / kFewRows);
   const size_t smem = warps * tiles * 8 * kFewRows * sizeof(float);
@@ -612,15 +615,19 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   int sms = 0;
   bool pair_ok = false;
   if (int rc = dense_setup(&sms, &pair_ok)) return rc;
-  if (!transpose_w && m <= kFewMaxCodeRows) {
+  // Few rows: 16 x 4096 x 2048 4.3 us against 7.6 us on the tensor-core tiles, 32 x 4096 x 2048 7.0 against 7.8 us; with 16 MB of weight the
+  // repeated reads of more than sixteen rows tell (32 x 4096 x 4096: 13.3 us against 9.1 us).
+  if (!transpose_w && (m <= kFewMaxRows || (m <= kFewMaxCodeRows && (uint64_t)n * k <= (1u << 23)))) {
     const FewArgs f = {a_fp8, a_pitch, a_scale_f32, a_scale_row_stride, a_scale_block_stride, (const uint8_t*)w_fp8, w_pitch, w_scale_f32,
                        w_scale_pitch, out, out_pitch, out_dtype, m, n, k};
-    return launch_few(f, 3, stream);
+    return launch_few(f, 3, sms, stream);
   }
   CUtensorMap tm_a, tm_w;
   if (int rc = encode_codes(&tm_a, a_fp8, m, k, a_pitch, 128)) return rc;
   const uint64_t m256 = (m + 255) / 256, n256 = (n + 255) / 256;
-  if (pair_ok && m256 * n256 * 2 > (uint64_t)sms * 3 / 4) {
+  // Pairs once one CTA per 128 x 128 tile no longer fits the device at once: 1024 x 2048 x 2048 (128 tiles) 10.4 us in one wave of
+  // single CTAs against 11.7 us in pairs, 1024 x 2560 x 2048 (160 tiles) 17.0 us against 12.4 us.
+  if (pair_ok && (uint64_t)((m + 127) / 128) * ((n + 127) / 128) > (uint64_t)sms) {
     if (m256 * n256 > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
     PairArgs p;
     p.a_scale = a_scale_f32; p.a_scale_row = a_scale_row_stride; p.a_scale_block = a_scale_block_stride;
@@ -682,15 +689,17 @@ int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, 
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < netra_dense_fp8_linear_workspace_bytes(m, k))
     return fail("dense_fp8_linear: workspace missing, too small or not 16-byte aligned");
   const uint64_t pitch = ((uint64_t)k + 15) / 16 * 16;
-  // few rows: the product quantises them itself, if whole 16-byte accesses fit them
-  if (!transpose_w && m <= kFewMaxRows && k % 8 == 0 && (uintptr_t)x % 16 == 0 && x_pitch * dense_element_bytes(dtype) % 16 == 0) {
+  // Few rows: the product quantises them itself, if whole 16-byte accesses fit them.  Every CTA reads all of them, so FP32 rows
+  // pay up to four (4 x 4096 x 2048: 5.4 us against 5.9 us with the quantiser's launch, 8 rows 7.6 us against 6.0 us), 16-bit ones up
+  // to sixteen (5.8 us against 6.3 us).
+  if (!transpose_w && m <= (dtype == kDenseF32 ? 4u : kFewMaxRows) && k % 8 == 0 && (uintptr_t)x % 16 == 0 && x_pitch * dense_element_bytes(dtype) % 16 == 0) {
     if (int rc = check_quantize_operands(x, dtype, x_pitch, m, k)) return rc;
     if (int rc = check_matmul_operands(out, dtype, out_pitch, w_fp8, w_pitch, w_scale_f32, w_scale_pitch, transpose_w, m, w_rows, w_cols)) return rc;
     int sms = 0;
     bool pair_ok = false;
     if (int rc = dense_setup(&sms, &pair_ok)) return rc;
     const FewArgs f = {x, x_pitch, nullptr, 0, 0, (const uint8_t*)w_fp8, w_pitch, w_scale_f32, w_scale_pitch, out, out_pitch, dtype, m, w_rows, k};
-    return launch_few(f, dtype, stream);
+    return launch_few(f, dtype, sms, stream);
   }
   uint8_t* codes = (uint8_t*)workspace;
   float* scale = (float*)(codes + (uint64_t)m * pitch);

@@ -183,6 +183,18 @@ def test_operand_layouts():
     assert torch.equal(dense.fp8_linear(t.t(), w, ws), dense.fp8_linear(x.cuda(), w, ws))
 
 
+@pytest.mark.parametrize("m,k", [(1, 1040), (5, 264), (16, 640), (17, 640), (32, 272), (33, 1040)])
+def test_alignment_of_the_activations_changes_nothing(m, k):
+    """Rows on any boundary take other accesses (and, for few rows, a quantiser launch of their own) to the same bits."""
+    g = torch.Generator().manual_seed(m)
+    for dtype in TYPES:
+        wide = torch.randn(m, k + 24, generator=g).to(dtype).cuda()
+        w, ws = make_weight(80, k, 6)
+        want = dense.fp8_linear(wide[:, 5:5 + k].clone(), w, ws)
+        assert torch.equal(dense.fp8_linear(wide[:, 5:5 + k], w, ws), want)
+        check_product(want, *quantize_definition(wide[:, 5:5 + k]), w, ws)
+
+
 def test_runs_repeat_and_zero_rows_stay_zero():
     g = torch.Generator().manual_seed(6)
     for m in (5, 40, 300):
