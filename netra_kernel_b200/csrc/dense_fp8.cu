@@ -42,6 +42,7 @@ __device__ __forceinline__ void begin_grid() {
 // lane, and let one lane store the block's four scales side by side (scales are stored block by block).
 // Scales go to scale[m * scale_row + b * scale_block].  kVector: eight columns are one aligned access and lie wholly inside
 // or outside the row.
+// 16384 x 2048: FP32 25.5 us = 6.6 TB/s, BF16 18.3 us = 5.6 TB/s (two rows a lane: 25.1 and 19.6 us, eight: 27.5 and 25.3 us).
 // ------------------------------------------------------------------------------------------
 template <typename T> struct DenseElement;
 template <> struct DenseElement<__nv_bfloat16> { static constexpr uint32_t code = kDenseBf16; };
@@ -122,9 +123,13 @@ netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8
   }
   if ((threadIdx.x & 15) == 0) {
     float* dst = scale + row0 * scale_row + b * scale_block;
+    if (kRows == 4 && scale_row == 1 && row0 + 4 <= m && (uintptr_t)dst % 16 == 0) {
+      *reinterpret_cast<float4*>(dst) = make_float4(s[0], s[1 % kRows], s[2 % kRows], s[3 % kRows]);
+    } else {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (row0 + r < m) dst[r * scale_row] = s[r];
+      for (int r = 0; r < kRows; ++r)
+        if (row0 + r < m) dst[r * scale_row] = s[r];
+    }
   }
 }
 
