@@ -202,6 +202,8 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, f
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory"); }
+
 // one look at a barrier by a whole warp
 __device__ __forceinline__ bool mbar_try_wait_warp(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -251,6 +253,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   const bool direct = ranks == 1 && g.out_vector == 2 && col0 + kBN <= g.n;
   const uint32_t kb0 = (uint32_t)((uint64_t)g.k_blocks * rank / ranks), kb1 = (uint32_t)((uint64_t)g.k_blocks * (rank + 1) / ranks);
 
+  if (threadIdx.x == 0 || threadIdx.x == 64) prefetch_tensormap(threadIdx.x == 0 ? &tm_a : &tm_w);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 2); mbar_init(smem_u32(&done_bar[s]), 1); }
     for (int a = 0; a < C::kAccStages; ++a) mbar_init(smem_u32(&tempty_bar[a]), 8);
@@ -307,25 +310,25 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
     float acc[kCols];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
-    // scales of eight K-blocks at a time, the next eight on their way: one at a time, their latency set the loop's pace
-    float s[8], ahead[8];
+    // scales of eight K-blocks at a time, the next eight asked for while the second of these is promoted: one at a time, their
+    // latency set the loop's pace
+    float sa[8], sw[8], sa_next[8], sw_next[8];
+    auto load_scales = [&](float to_a[8], float to_w[8], uint32_t from) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t kb = min(kb0 + j, g.k_blocks - 1);
-      s[j] = __ldcg(sa_ptr + kb * g.a_scale_block) * __ldcg(sw_ptr + kb * g.w_scale_block);
-    }
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t kb = min(from + j, g.k_blocks - 1);
+        to_a[j] = __ldcg(sa_ptr + kb * g.a_scale_block);
+        to_w[j] = __ldcg(sw_ptr + kb * g.w_scale_block);
+      }
+    };
+    load_scales(sa, sw, kb0);
     bool ok = true;
     for (uint32_t base = kb0; ok && base < kb1; base += 8) {
-      if (base + 8 < kb1) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t kb = min(base + 8 + j, g.k_blocks - 1);
-          ahead[j] = __ldcg(sa_ptr + kb * g.a_scale_block) * __ldcg(sw_ptr + kb * g.w_scale_block);
-        }
-      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (!ok || base + j >= kb1) break;
+        if (j == 1 && base + 8 < kb1) load_scales(sa_next, sw_next, base + 8);
+        const float s = __fmul_rn(sa[j], sw[j]);
         const uint32_t it = base + j - kb0, a = it % C::kAccStages;
         if (!mbar_wait_warp(smem_u32(&done_bar[it % C::kStages]), (it / C::kStages) & 1, abort_flag)) {
           g_dense_status[0] = kStatusEpilogueTimeout; *abort_flag = 1; ok = false; break;
@@ -342,10 +345,10 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
 #pragma unroll
         for (int q = 0; q < kCols / 32; ++q)
 #pragma unroll
-          for (int c = 0; c < 32; ++c) acc[32 * q + c] = fmaf(__uint_as_float(v[q][c]), s[j], acc[32 * q + c]);
+          for (int c = 0; c < 32; ++c) acc[32 * q + c] = fmaf(__uint_as_float(v[q][c]), s, acc[32 * q + c]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = ahead[j];
+      for (int j = 0; j < 8; ++j) { sa[j] = sa_next[j]; sw[j] = sw_next[j]; }
     }
     if (direct) {
       if (row < g.m) {
@@ -390,24 +393,18 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   const uint32_t share = 128u / ranks, first = row0 + rank * share;
   if (first >= g.m) return;
   const uint32_t count = min(share, g.m - first);
-  auto sum_at = [&](uint32_t r, uint32_t c, auto& to) {
-    using V = std::remove_reference_t<decltype(to)>;
-    const float* p = parts + (size_t)r * C::kOutPitch + c;
-    to = *reinterpret_cast<const V*>(p);
-    for (uint32_t j = 1; j < ranks; ++j) {
-      const V q = *reinterpret_cast<const V*>(p + (size_t)j * share * C::kOutPitch);
-      if constexpr (sizeof(V) == 16) { to.x += q.x; to.y += q.y; to.z += q.z; to.w += q.w; }
-      else to += q;
-    }
-  };
   if (g.out_vector && col0 + kBN <= g.n) {
     // a quarter, half or whole warp takes a row, a lane four neighbouring columns
     constexpr uint32_t kLanes = kBN / 4, kRowsAtOnce = kDnThreads / kLanes;
     const uint32_t c = (threadIdx.x % kLanes) * 4;
 #pragma unroll 4
     for (uint32_t r = threadIdx.x / kLanes; r < count; r += kRowsAtOnce) {
-      float4 v;
-      sum_at(r, c, v);
+      const float* p = parts + (size_t)r * C::kOutPitch + c;
+      float4 v = *reinterpret_cast<const float4*>(p);
+      for (uint32_t j = 1; j < ranks; ++j) {
+        const float4 q = *reinterpret_cast<const float4*>(p + (size_t)j * share * C::kOutPitch);
+        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+      }
       const uint64_t at = (uint64_t)(first + r) * g.out_pitch + col0 + c;
       if (g.out_dtype == kDenseF32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + at) = v;
       else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.out) + at) = make_uint2(pack_16bit(g.out_dtype, v.x, v.y), pack_16bit(g.out_dtype, v.z, v.w));
@@ -415,15 +412,37 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
   } else {
     // rows on any boundary, or a tile that ends inside: neighbouring lanes store neighbouring elements
     const uint32_t cols = min((uint32_t)kBN, g.n - col0);
-    for (uint32_t r = warp; r < count; r += kDnThreads / 32) {
+    constexpr int kRowsAtOnce = 4, kPerLane = kBN / 32, kWarps = kDnThreads / 32;
+    auto store_rows = [&](auto element) {
+      using T = decltype(element);
+      T* to = reinterpret_cast<T*>(g.out) + (uint64_t)first * g.out_pitch + col0 + lane;
+      for (uint32_t r0 = warp; r0 < count; r0 += kRowsAtOnce * kWarps) {
+        float v[kRowsAtOnce][kPerLane];
+        const float* p = parts + (size_t)r0 * C::kOutPitch + lane;     // rows past the share are summed in place and not stored
 #pragma unroll
-      for (uint32_t c = lane; c < (uint32_t)kBN; c += 32) {
-        if (c >= cols) continue;
-        float v;
-        sum_at(r, c, v);
-        dense_store(g.out, g.out_dtype, (uint64_t)(first + r) * g.out_pitch + col0 + c, v);
+        for (int i = 0; i < kRowsAtOnce; ++i)
+#pragma unroll
+          for (int j = 0; j < kPerLane; ++j) v[i][j] = r0 + i * kWarps < share ? p[i * kWarps * C::kOutPitch + 32 * j] : 0.0f;
+        for (uint32_t q = 1; q < ranks; ++q) {
+          p += (size_t)share * C::kOutPitch;
+#pragma unroll
+          for (int i = 0; i < kRowsAtOnce; ++i)
+#pragma unroll
+            for (int j = 0; j < kPerLane; ++j)
+              if (r0 + i * kWarps < share) v[i][j] += p[i * kWarps * C::kOutPitch + 32 * j];
+        }
+#pragma unroll
+        for (int i = 0; i < kRowsAtOnce; ++i) {
+          if (r0 + i * kWarps >= count) break;
+#pragma unroll
+          for (int j = 0; j < kPerLane; ++j)
+            if (lane + 32 * j < cols) dense_store(to + (uint64_t)(r0 + i * kWarps) * g.out_pitch, DenseElement<T>::code, 32 * j, v[i][j]);
+        }
       }
-    }
+    };
+    if (g.out_dtype == kDenseF32) store_rows(0.0f);
+    else if (g.out_dtype == kDenseF16) store_rows(__half{});
+    else store_rows(__nv_bfloat16{});
   }
 }
 

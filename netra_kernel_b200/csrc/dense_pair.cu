@@ -121,6 +121,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
   const uint32_t rank = cluster_rank();
   const uint32_t items = g.m_tiles * g.n_tiles, pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
 
+  if (threadIdx.x < 96 && lane == 0) prefetch_tensormap(warp == 0 ? &tm_a : warp == 1 ? &tm_w : &tm_out);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&done_bar[2 * s]), 2); mbar_init(smem_u32(&done_bar[2 * s + 1]), 2); }
     for (int a = 0; a < 4; ++a) mbar_init(smem_u32(&tempty_bar[a]), rank == 0 ? 9 : 8);     // promotion warps, and the peer's relay
