@@ -121,15 +121,23 @@ struct BalLane {
       }
     }
   }
-  // the counts of the lane's experts; returns 1 / their sum over the warp (FP32: a common factor, off by a few steps at most)
-  __device__ static __forceinline__ float counts(float c[kPer], const int32_t* __restrict__ all, uint32_t experts, int lane) {
+  // The counts of the lane's experts above the smallest count, which goes to least: f_e - d_t, small when the load is nearly
+  // even, then comes from whole numbers as small (and is exactly 0 when it is even).  Returns 1 / the sum of the counts (FP32: a
+  // common factor, off by a few steps at most).
+  __device__ static __forceinline__ float counts(float c[kPer], float& least, const int32_t* __restrict__ all, uint32_t experts, int lane) {
+    int n[kPer], low = 0x7fffffff;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const uint32_t e = expert(i, lane);
-      c[i] = e < experts ? (float)__ldg(all + e) : 0.0f;
-      sum += c[i];
+      n[i] = e < experts ? __ldg(all + e) : 0x7fffffff;
+      if (e < experts) sum += (float)n[i];
+      low = min(low, n[i]);
     }
+    low = __reduce_min_sync(0xffffffffu, low);
+    least = (float)low;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c[i] = expert(i, lane) < experts ? (float)(n[i] - low) : 0.0f;
     sum = warp_sum(sum);
     return sum > 0.0f ? 1.0f / sum : 0.0f;
   }
@@ -188,12 +196,13 @@ __device__ __forceinline__ void balance_loss_body(const T* __restrict__ z, uint6
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double sum = 0.0;
   unsigned long long rows = 0;
-  float c[kPer], v[kPer], inv;
-  const float per_count = L::counts(c, counts, experts, lane);
+  float c[kPer], v[kPer], inv, least;
+  const float per_count = L::counts(c, least, counts, experts, lane);
   for (uint64_t t = (uint64_t)blockIdx.x * kWarps + warp; t < tokens; t += (uint64_t)gridDim.x * kWarps) {
     if (mask != nullptr && mask[t] == 0) continue;
     L::load(v, z + t * pitch, experts, lane);
-    sum += (double)(bal_row<kPer>(v, c, inv) * per_count);
+    const float above = bal_row<kPer>(v, c, inv);
+    sum += inv == 0.0f ? 0.0 : (double)((least + above) * per_count);
     ++rows;
   }
   if (lane == 0) { warp_part[warp] = sum; warp_rows[warp] = rows; }
@@ -268,8 +277,8 @@ netra_balance_loss_grad_sm100(T* __restrict__ grad, uint64_t grad_pitch, const T
   using L = BalLane<T, kAligned, kPer>;
   begin_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float c[kPer], v[kPer], inv;
-  const float per_count = L::counts(c, counts, experts, lane);
+  float c[kPer], v[kPer], inv, least;
+  const float per_count = L::counts(c, least, counts, experts, lane);
   const float k = *scale * *upstream;
   for (uint64_t t = (uint64_t)blockIdx.x * (kBalThreads / 32) + warp; t < tokens; t += (uint64_t)gridDim.x * (kBalThreads / 32)) {
     if (mask == nullptr || mask[t] != 0) {

@@ -117,6 +117,25 @@ def test_masked_experts_and_rows(dtype):
     assert loss.item() == 0.0 and bool((dz == 0).all())
 
 
+def test_even_and_nearly_even_loads():
+    """An even load has no gradient at all; one choice more or less gives a gradient as exact as the small difference it comes
+    from (counts up to 2^24 are whole numbers in FP32)."""
+    g = torch.Generator().manual_seed(6)
+    z = torch.randn(50, 64, generator=g).cuda().requires_grad_()
+    even = torch.full((64,), 123457, dtype=torch.int32, device="cuda")
+    loss = balance.balance_loss(z, even)
+    (grad,) = torch.autograd.grad(loss, z)
+    assert abs(loss.item() - 1.0) <= 40 * 2.0 ** -23 and bool((grad == 0).all())
+    even[3] += 1
+    even[9] -= 2
+    loss, grad, _, u = definition(z, even, None)
+    (got,) = torch.autograd.grad(balance.balance_loss(z, even), z)
+    c = even.cpu().double() - even.min().item()
+    p = torch.softmax(z.detach().cpu().double(), dim=1)
+    size = 64 / 50 * p * (c + (p @ c)[:, None]) / even.sum().item()
+    assert bool(((got.cpu().double() - grad).abs() <= 3 * u[:, None] * size + 1e-37).all())
+
+
 def test_layouts_and_empty_batches():
     g = torch.Generator().manual_seed(3)
     base = torch.randn(64, 300, generator=g).cuda()
