@@ -300,9 +300,9 @@ netra_balance_loss_grad_sm100(T* __restrict__ grad, uint64_t grad_pitch, const T
 namespace {
 
 // Up to here one cluster of eight blocks does it, without clearing anything first (one cluster against many blocks behind a
-// memset: counts of 2,048 choices 2.7 us against 5.0 us, of 131,072 choices 5.9 us against 6.2 us; loss of 256 tokens and 256
+// memset: counts of 2,048 choices 2.7 us against 5.0 us, of 65,536 choices 4.8 us against 6.2 us; loss of 256 tokens and 256
 // experts 3.3 us against 6.4 us, of 2,048 tokens 8.1 us each, of 4,096 tokens 13.4 us against 8.4 us).
-constexpr uint64_t kCountsClusterPairs = 1 << 17, kLossClusterTokens = 2048;
+constexpr uint64_t kCountsClusterPairs = 1 << 16, kLossClusterTokens = 2048;
 constexpr uint32_t kBalMaxBlocks = 592;       // four blocks per SM of a 148-SM device: more warps only repeat the look at the counts
 
 int balance_check(const char* what, const void* z, uint32_t dtype, uint64_t pitch, const void* counts, uint64_t tokens, uint32_t experts) {

@@ -63,7 +63,7 @@ void check_weight_on(const Tensor& w, const Tensor& s, const at::Device& device)
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& input) {
   const Tensor x = as_rows(input.detach(), "x");
-  const int64_t m = x.size(0), k = x.size(1), pitch = ceil_div(k, 16) * 16, blocks = ceil_div(k, kBlockCols);
+  const int64_t m = x.size(0), k = x.size(1), blocks = ceil_div(k, kBlockCols), pitch = blocks * kBlockCols;
   Tensor codes = at::empty({m, pitch}, x.options().dtype(at::kFloat8_e4m3fn));
   Tensor scale = at::empty_strided({m, blocks}, {1, std::max<int64_t>(m, 1)}, x.options().dtype(at::kFloat));
   if (m > 0) {

@@ -29,7 +29,7 @@ BLOCK = 128
 def quantize_rows(x: torch.Tensor):
     """``x`` [..., K] (BF16, FP16 or FP32) -> (E4M3 codes [M, K], FP32 scales [M, ceil(K/128)]), M the product of the leading
     sizes: ``scale = max(amax of the row's 128 columns, 1e-10) * fl(1/448)``, ``code = e4m3_rne_sat(x * fl(1/scale))``.
-    The rows of the codes are padded to 16 bytes and the scales stored block by block, the forms the product reads best.
+    The rows of the codes are padded to 128 bytes and the scales stored block by block, the forms the product reads best.
     A NaN stays at its element; an infinity makes its block's scale infinite."""
     return _ext.quantize_rows(x)
 
