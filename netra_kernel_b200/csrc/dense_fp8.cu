@@ -692,12 +692,17 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   g.out_vector = ((uintptr_t)out | out_pitch * out_bytes) % 32 == 0 ? 2 : (uintptr_t)out % (4 * out_bytes) == 0 && out_pitch % 4 == 0 ? 1 : 0;
   g.m = m; g.n = n; g.k_blocks = (k + 127) / 128;
   const uint64_t m_tiles = (m + 127) / 128;
-  const bool narrow = !transpose_w && m_tiles * ((n + 127) / 128) * 2 <= (uint64_t)sms;
+  // 64 columns a tile while that still is one wave (256 x 4096 x 2048: 9.1 us against 10.5 us with 128), or where there are no more
+  // (16384 x 64 x 2048: 9.7 us against 11.9 us).  The gradient's weight tile is one swizzle atom of 128 columns.
+  const bool narrow = !transpose_w && (n <= 64 || m_tiles * ((n + 127) / 128) * 2 <= (uint64_t)sms);
   const uint32_t bn = narrow ? 64 : 128;
   g.n_tiles = (n + bn - 1) / bn;
   const uint64_t tiles = m_tiles * g.n_tiles;
   uint32_t split = 1;
-  while (split < 8 && tiles * split * 2 <= (uint64_t)sms && g.k_blocks >= split * 4) split *= 2;
+  // Eight K-blocks and more for every CTA of a cluster (128 x 1024 x 1024: 4.6 us as it is, 5.4 us in two, 6.0 us in four).  Clusters of
+  // eight only where few are needed: a GPC holds two of them at one CTA an SM, and a second wave doubles the time (64 x 1024 x 4096:
+  // sixteen clusters of eight 11.7 us, of four 6.6 us).
+  while (split < (tiles <= 8 ? 8u : 4u) && tiles * split * 2 <= (uint64_t)sms && g.k_blocks >= split * 16) split *= 2;
   if (tiles * split > 0x7fffffffull) return fail("dense_fp8_matmul: too many output tiles in one call");
   if (int rc = encode_codes(&tm_w, w_fp8, w_rows, w_cols, w_pitch, transpose_w ? 128 : bn)) return rc;
   const dim3 grid((unsigned)(tiles * split));
