@@ -560,12 +560,14 @@ constexpr uint32_t kFewMaxRows = 16, kFewMaxCodeRows = 32;
 
 // Product of few rows; x of type code `source` (kDense*, or 3 for codes with their scales).
 int launch_few(const FewArgs& g, uint32_t source, int sms, cudaStream_t stream) {
-  // two K-blocks a warp at first; sixteen warps, or eight where two CTAs an SM overlap their starts and ends (1 x 8192 x 8192:
-  // 17.9 us with sixteen, 16.0 us with eight; 1 x 4096 x 4096: 5.8 us against 6.1 us)
-  const uint32_t blocks = (g.k + 127) / 128, most = (g.n + kFewRows - 1) / kFewRows > 2u * (uint32_t)sms ? 8 : 16;
-  const uint32_t warps = (blocks + 1) / 2 < most ? (blocks + 1) / 2 : most;
+  // One K-block a warp where every CTA has an SM to itself (16 x 1024 x 1024: 2.7 us, with two a warp 3.4 us), two where they share
+  // (16 x 4096 x 2048: 5.6 us with one, 4.4 us with two).  Sixteen warps at most, or eight where more CTAs follow, whose starts then
+  // overlap the others' ends (1 x 8192 x 8192: 17.9 us with sixteen, 16.0 us with eight).
+  const uint32_t blocks = (g.k + 127) / 128, ctas = (g.n + kFewRows - 1) / kFewRows;
+  const uint32_t most = ctas > 2u * (uint32_t)sms ? 8 : 16, wanted = ctas <= (uint32_t)sms ? blocks : (blocks + 1) / 2;
+  const uint32_t warps = wanted < most ? wanted : most;
   const uint32_t tiles = g.m <= 8 ? 1 : g.m <= 16 ? 2 : 4;
-  const dim3 grid((g.n + kFewRows - 1) / kFewRows);
+  const dim3 grid(ctas);
   const size_t smem = warps * tiles * 8 * kFewRows * sizeof(float);
   auto launch = [&](auto element) {
     using T = decltype(element);
@@ -647,9 +649,10 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
   int sms = 0;
   bool pair_ok = false;
   if (int rc = dense_setup(&sms, &pair_ok)) return rc;
-  // Few rows: 16 x 4096 x 2048 4.3 us against 7.6 us on the tensor-core tiles, 32 x 4096 x 2048 7.0 against 7.8 us; with 16 MB of weight the
-  // repeated reads of more than sixteen rows tell (32 x 4096 x 4096: 13.3 us against 9.1 us).
-  if (!transpose_w && (m <= kFewMaxRows || (m <= kFewMaxCodeRows && (uint64_t)n * k <= (1u << 23)))) {
+  // Few rows: 16 x 4096 x 2048 4.4 us against 7.4 us on the tensor-core tiles.  More than sixteen are read again by every CTA, which
+  // pays while each has an SM to itself and the weight is small (17 x 2048 x 2048: 4.1 us against 7.1 us, 32 x 512 x 1024: 3.7 us
+  // against 4.1 us; but 32 x 2048 x 4096 7.6 us against 7.3 us, 32 x 4096 x 4096 13.3 us against 9.1 us).
+  if (!transpose_w && (m <= kFewMaxRows || (m <= kFewMaxCodeRows && n <= (uint32_t)sms * kFewRows && (uint64_t)n * k <= (1u << 22)))) {
     const FewArgs f = {a_fp8, a_pitch, a_scale_f32, a_scale_row_stride, a_scale_block_stride, (const uint8_t*)w_fp8, w_pitch, w_scale_f32,
                        w_scale_pitch, out, out_pitch, out_dtype, m, n, k};
     return launch_few(f, 3, sms, stream);
