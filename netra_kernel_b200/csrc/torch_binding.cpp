@@ -64,7 +64,7 @@ void check_weight_on(const Tensor& w, const Tensor& s, const at::Device& device)
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& input) {
   const Tensor x = as_rows(input.detach(), "x");
   const int64_t m = x.size(0), k = x.size(1), blocks = ceil_div(k, kBlockCols), pitch = blocks * kBlockCols;
-  Tensor codes = at::empty({m, pitch}, x.options().dtype(at::kFloat8_e4m3fn));
+  Tensor codes = at::empty_strided({m, k}, {pitch, 1}, x.options().dtype(at::kFloat8_e4m3fn));
   Tensor scale = at::empty_strided({m, blocks}, {1, std::max<int64_t>(m, 1)}, x.options().dtype(at::kFloat));
   if (m > 0) {
     const c10::cuda::CUDAGuard guard(x.device());
@@ -72,7 +72,7 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& input) {
                                               pitch_of(x), (uint32_t)m, (uint32_t)k, stream_of(x)),
              "dense_quantize_rows_launch");
   }
-  return {pitch == k ? codes : codes.narrow(1, 0, k), scale};
+  return {codes, scale};
 }
 
 void check_sizes(int64_t m, const Tensor& w) {
