@@ -44,14 +44,17 @@ Tensor as_rows(const Tensor& x, const char* what) {
   return r;
 }
 
-// an element pitch the C ABI accepts: a single row may report any stride
+// element pitches the C ABI accepts: a single row may report any stride
 uint64_t pitch_of(const Tensor& t) { return (uint64_t)std::max(t.stride(0), t.size(1)); }
+uint64_t code_pitch_of(const Tensor& t) { return (uint64_t)(t.size(0) > 1 ? t.stride(0) : ceil_div(t.size(1), 16) * 16); }
+
+constexpr int64_t kMaxSize = 1 << 26;
 
 void check_weight(const Tensor& w, const Tensor& s, const at::Device& device) {
   TORCH_CHECK_VALUE(w.device() == device && s.device() == device, "weight and weight_scale must be on the activations' device");
   TORCH_CHECK_VALUE(w.scalar_type() == at::kFloat8_e4m3fn && w.dim() == 2 && w.numel() > 0, "weight must be float8_e4m3fn [N, K]");
   const int64_t n = w.size(0), k = w.size(1);
-  TORCH_CHECK_VALUE((w.stride(1) == 1 || k == 1) && w.stride(0) % 16 == 0 && w.stride(0) >= k && (uintptr_t)w.const_data_ptr() % 16 == 0,
+  TORCH_CHECK_VALUE((w.stride(1) == 1 || k == 1) && (n == 1 || (w.stride(0) % 16 == 0 && w.stride(0) >= k)) && (uintptr_t)w.const_data_ptr() % 16 == 0,
                     "weight rows must be contiguous and start on 16-byte boundaries");
   TORCH_CHECK_VALUE(s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == ceil_div(n, kBlockCols) && s.size(1) == ceil_div(k, kBlockCols),
                     "weight_scale must be float32 [ceil(N/128), ceil(K/128)]");
@@ -63,6 +66,7 @@ void check_weight_on(const Tensor& w, const Tensor& s, const at::Device& device)
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& input) {
   const Tensor x = as_rows(input.detach(), "x");
+  TORCH_CHECK_VALUE(x.size(0) <= kMaxSize && x.size(1) <= kMaxSize, "sizes must not exceed 2^26");
   const int64_t m = x.size(0), k = x.size(1), blocks = ceil_div(k, kBlockCols), pitch = blocks * kBlockCols;
   Tensor codes = at::empty_strided({m, k}, {pitch, 1}, x.options().dtype(at::kFloat8_e4m3fn));
   Tensor scale = at::empty_strided({m, blocks}, {1, std::max<int64_t>(m, 1)}, x.options().dtype(at::kFloat));
@@ -76,7 +80,7 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& input) {
 }
 
 void check_sizes(int64_t m, const Tensor& w) {
-  TORCH_CHECK_VALUE(m <= (1 << 26) && w.size(0) <= (1 << 26) && w.size(1) <= (1 << 26), "sizes must not exceed 2^26");
+  TORCH_CHECK_VALUE(m <= kMaxSize && w.size(0) <= kMaxSize && w.size(1) <= kMaxSize, "sizes must not exceed 2^26");
 }
 
 Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& w, const Tensor& ws, bool transpose_weight,
@@ -102,9 +106,8 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
   }
   if (m > 0) {
     const c10::cuda::CUDAGuard guard(a.device());
-    const uint64_t a_pitch = m > 1 ? a.stride(0) : ceil_div(k, 16) * 16;
-    check_rc(netra_dense_fp8_matmul_launch(out.data_ptr(), element_code(out.scalar_type()), pitch_of(out), a.const_data_ptr(), a_pitch,
-                                           a_scale.const_data_ptr<float>(), a_scale.stride(0), a_scale.stride(1), w.const_data_ptr(), w.stride(0),
+    check_rc(netra_dense_fp8_matmul_launch(out.data_ptr(), element_code(out.scalar_type()), pitch_of(out), a.const_data_ptr(), code_pitch_of(a),
+                                           a_scale.const_data_ptr<float>(), a_scale.stride(0), a_scale.stride(1), w.const_data_ptr(), code_pitch_of(w),
                                            ws.const_data_ptr<float>(), pitch_of(ws), transpose_weight, (uint32_t)m, (uint32_t)w.size(0),
                                            (uint32_t)w.size(1), stream_of(a)),
              "dense_fp8_matmul_launch");
@@ -122,7 +125,7 @@ Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool trans
     const uint64_t bytes = netra_dense_fp8_linear_workspace_bytes((uint32_t)m, (uint32_t)k);
     const Tensor workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
     check_rc(netra_dense_fp8_linear_launch(out.data_ptr(), n, x.const_data_ptr(), element_code(x.scalar_type()), pitch_of(x), w.const_data_ptr(),
-                                           w.stride(0), ws.const_data_ptr<float>(), pitch_of(ws), transposed, (uint32_t)m, (uint32_t)w.size(0),
+                                           code_pitch_of(w), ws.const_data_ptr<float>(), pitch_of(ws), transposed, (uint32_t)m, (uint32_t)w.size(0),
                                            (uint32_t)w.size(1), workspace.data_ptr(), bytes, stream_of(x)),
              "dense_fp8_linear_launch");
   }

@@ -29,6 +29,7 @@ def test_weight_checks():
     ok, scale = _fp8(300, 272), torch.ones(3, 3)
     abi.torch_binding().check_weight(ok, scale, cpu)
     abi.torch_binding().check_weight(_fp8(300, 288)[:, :260], scale, cpu)                    # padded rows
+    abi.torch_binding().check_weight(_fp8(1, 260), torch.ones(1, 3), cpu)                    # a single row has no pitch
     for weight, s, why in [
         (ok.view(torch.uint8), scale, "float8"), (_fp8(0, 128), torch.ones(0, 1), "float8"),
         (_fp8(300, 260), scale, "16-byte"), (ok.t(), torch.ones(3, 3), "16-byte"), (_fp8(301, 272).view(-1)[16 * 17 - 8:-8].view(300, 272), scale, "16-byte"),

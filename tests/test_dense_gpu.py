@@ -63,7 +63,8 @@ def check_product(y, q, s, w, ws, transposed=False):
 
 SIZES = [(1, 16, 16), (1, 2048, 4096), (2, 1, 128), (3, 129, 112), (7, 64, 144), (8, 300, 1040), (9, 65, 128), (12, 512, 2048),
          (16, 127, 256), (17, 128, 384), (31, 1043, 272), (33, 96, 4112), (64, 256, 512), (100, 63, 640), (127, 192, 128), (128, 128, 128),
-         (129, 257, 2064), (200, 2048, 512), (257, 512, 1024), (300, 80, 16), (777, 1043, 2064), (1024, 640, 384), (1500, 1280, 256)]
+         (129, 257, 2064), (200, 2048, 512), (257, 512, 1024), (300, 80, 16), (777, 1043, 2064), (1024, 640, 384), (1500, 1280, 256),
+         (1, 1, 1), (4, 1, 260), (5, 33, 77), (20, 200, 131), (140, 97, 1001), (64, 2048, 2048), (40, 130, 16400), (130, 1, 4100)]
 
 
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 128), (3, 7), (5, 130), (16, 1000), (33, 2048), (257, 144), (64, 4112), (2000, 640)])
@@ -215,9 +216,14 @@ def test_gradient_is_the_formula(m, n, k, dtype):
     w, ws = make_weight(n, k, n)
     dy = (torch.randn(m, n, generator=g) * 0.3).to(dtype)
     y = dense.fp8_linear(x, w, ws)
+    deep = x.detach().view(1, m, 1, k).requires_grad_()
+    (deep_dx,) = torch.autograd.grad(dense.fp8_linear(deep, w, ws), deep, dy.cuda().view(1, m, 1, n))
+    (none,) = torch.autograd.grad(dense.fp8_linear(x[:0], w, ws).sum(), x)
+    assert bool((none == 0).all())
     (dx,) = torch.autograd.grad(y, x, dy.cuda())
     assert dx.dtype == dtype
     check_product(dx, *quantize_definition(dy), w, ws, True)
+    assert deep_dx.shape == deep.shape and torch.equal(deep_dx.view(m, k), dx)
     (dx2,) = torch.autograd.grad(dense.fp8_linear(x, w, ws).sum(), x)        # an expanded gradient
     check_product(dx2, *quantize_definition(torch.ones(m, n).to(dtype)), w, ws, True)
     with torch.no_grad():
@@ -280,6 +286,19 @@ def test_streams_and_captured_graphs():
         torch.cuda.synchronize()
         y = dense.fp8_linear(static, w, ws)
         assert torch.equal(outs[0], y) and torch.equal(outs[1], y)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()          # a fork and a join inside one graph
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            left = dense.fp8_linear(static, w, ws)
+        right = dense.fp8_linear(xs[2], w, ws)
+        torch.cuda.current_stream().wait_stream(side)
+        both = dense.fp8_linear(torch.cat([left, right])[:, :256].contiguous(), w[:, :256], ws[:, :2])
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(left, dense.fp8_linear(static, w, ws)) and torch.equal(right, want[2])
+    assert torch.equal(both, dense.fp8_linear(torch.cat([left, right])[:, :256].contiguous(), w[:, :256], ws[:, :2]))
     leaf = xs[1].clone().requires_grad_()
     dy = torch.randn(90, 512, generator=g).to(torch.bfloat16).cuda()
     (eager,) = torch.autograd.grad(dense.fp8_linear(leaf, w, ws), leaf, dy)
