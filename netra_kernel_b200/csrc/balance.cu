@@ -16,8 +16,8 @@ constexpr int kBalCluster = 8;            // blocks of the one-cluster forms
 constexpr int kBalClusterThreads = 1024;
 
 // hist[e] += the block's share of the choices: blocks first, first + step, ... of blockDim choices each
-__device__ __forceinline__ void count_choices(int* hist, const void* __restrict__ ids, uint32_t wide, uint64_t id_pitch,
-                                              const uint8_t* __restrict__ mask, uint64_t tokens, uint32_t slots, uint32_t experts) {
+__device__ __forceinline__ void count_choices(int* hist, const void* ids, uint32_t wide, uint64_t id_pitch,
+                                              const uint8_t* mask, uint64_t tokens, uint32_t slots, uint32_t experts) {
   for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
   const uint32_t pairs = (uint32_t)tokens * slots, step = gridDim.x * blockDim.x;       // the host keeps pairs below 2^31
@@ -34,8 +34,8 @@ __device__ __forceinline__ void count_choices(int* hist, const void* __restrict_
 
 // ids [tokens, slots] (rows id_pitch apart) -> counts [experts], which the caller cleared
 extern "C" __global__ void __launch_bounds__(256)
-netra_expert_counts_sm100(const void* __restrict__ ids, uint32_t wide, uint64_t id_pitch, const uint8_t* __restrict__ mask,
-                          int32_t* __restrict__ counts, uint64_t tokens, uint32_t slots, uint32_t experts) {
+netra_expert_counts_sm100(const void* ids, uint32_t wide, uint64_t id_pitch, const uint8_t* mask,
+                          int32_t* counts, uint64_t tokens, uint32_t slots, uint32_t experts) {
   __shared__ int hist[kBalMaxExperts];
   begin_grid();
   count_choices(hist, ids, wide, id_pitch, mask, tokens, slots, experts);
@@ -45,8 +45,8 @@ netra_expert_counts_sm100(const void* __restrict__ ids, uint32_t wide, uint64_t 
 
 // The same in one cluster, whose blocks add up their histograms over distributed shared memory: nothing to clear beforehand
 extern "C" __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalClusterThreads)
-netra_expert_counts_cluster_sm100(const void* __restrict__ ids, uint32_t wide, uint64_t id_pitch, const uint8_t* __restrict__ mask,
-                                  int32_t* __restrict__ counts, uint64_t tokens, uint32_t slots, uint32_t experts) {
+netra_expert_counts_cluster_sm100(const void* ids, uint32_t wide, uint64_t id_pitch, const uint8_t* mask,
+                                  int32_t* counts, uint64_t tokens, uint32_t slots, uint32_t experts) {
   __shared__ int hist[kBalMaxExperts];
   begin_grid();
   count_choices(hist, ids, wide, id_pitch, mask, tokens, slots, experts);
@@ -76,7 +76,7 @@ struct BalLane {
   static constexpr int kVec = 16 / sizeof(T);
   static_assert(kPer % kVec == 0, "a lane holds whole accesses");
   __device__ static __forceinline__ uint32_t expert(int i, int lane) { return (uint32_t)((i / kVec) * 32 * kVec + lane * kVec + i % kVec); }
-  __device__ static __forceinline__ void load(float v[kPer], const T* __restrict__ row, uint32_t experts, int lane) {
+  __device__ static __forceinline__ void load(float v[kPer], const T* row, uint32_t experts, int lane) {
 #pragma unroll
     for (int i = 0; i < kPer; i += kVec) {
       const uint32_t e = expert(i, lane);
@@ -93,7 +93,7 @@ struct BalLane {
       }
     }
   }
-  __device__ static __forceinline__ void store(T* __restrict__ row, const float v[kPer], uint32_t experts, int lane) {
+  __device__ static __forceinline__ void store(T* row, const float v[kPer], uint32_t experts, int lane) {
 #pragma unroll
     for (int i = 0; i < kPer; i += kVec) {
       const uint32_t e = expert(i, lane);
@@ -124,13 +124,13 @@ struct BalLane {
   // The counts of the lane's experts above the smallest count, which goes to least: f_e - d_t, small when the load is nearly
   // even, then comes from whole numbers as small (and is exactly 0 when it is even).  Returns 1 / the sum of the counts (FP32: a
   // common factor, off by a few steps at most).
-  __device__ static __forceinline__ float counts(float c[kPer], float& least, const int32_t* __restrict__ all, uint32_t experts, int lane) {
+  __device__ static __forceinline__ float counts(float c[kPer], float& least, const int32_t* all, uint32_t experts, int lane) {
     int n[kPer], low = 0x7fffffff;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const uint32_t e = expert(i, lane);
-      n[i] = e < experts ? __ldg(all + e) : 0x7fffffff;
+      n[i] = e < experts ? all[e] : 0x7fffffff;
       if (e < experts) sum += (float)n[i];
       low = min(low, n[i]);
     }
@@ -181,9 +181,9 @@ struct BalPartial { double sum; unsigned long long rows; };
 // kCluster: the grid is one cluster, whose blocks leave their sums in the first one's shared memory; otherwise partial has one
 // slot per block, and the block that draws the last number of ticket (cleared by the caller) adds them up.
 template <typename T, bool kAligned, int kPer, bool kCluster>
-__device__ __forceinline__ void balance_loss_body(const T* __restrict__ z, uint64_t pitch, const int32_t* __restrict__ counts,
-                                                  const uint8_t* __restrict__ mask, float* __restrict__ loss, float* __restrict__ scale,
-                                                  BalPartial* __restrict__ partial, uint32_t* __restrict__ ticket, uint64_t tokens,
+__device__ __forceinline__ void balance_loss_body(const T* z, uint64_t pitch, const int32_t* counts,
+                                                  const uint8_t* mask, float* loss, float* scale,
+                                                  BalPartial* partial, uint32_t* ticket, uint64_t tokens,
                                                   uint32_t experts) {
   using L = BalLane<T, kAligned, kPer>;
   constexpr int kWarps = (kCluster ? kBalClusterThreads : kBalThreads) / 32;
@@ -271,9 +271,9 @@ netra_balance_loss_cluster_sm100(const T* z, uint64_t pitch, const int32_t* coun
 
 template <typename T, bool kAligned, int kPer>
 __global__ void __launch_bounds__(kBalThreads)
-netra_balance_loss_grad_sm100(T* __restrict__ grad, uint64_t grad_pitch, const T* __restrict__ z, uint64_t pitch,
-                              const int32_t* __restrict__ counts, const uint8_t* __restrict__ mask, const float* __restrict__ scale,
-                              const float* __restrict__ upstream, uint64_t tokens, uint32_t experts) {
+netra_balance_loss_grad_sm100(T* grad, uint64_t grad_pitch, const T* z, uint64_t pitch,
+                              const int32_t* counts, const uint8_t* mask, const float* scale,
+                              const float* upstream, uint64_t tokens, uint32_t experts) {
   using L = BalLane<T, kAligned, kPer>;
   begin_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

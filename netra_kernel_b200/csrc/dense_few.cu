@@ -20,7 +20,7 @@ __device__ __forceinline__ void mma_e4m3_16x8x32(float c[4], uint32_t a0, uint32
 }
 
 // 16 codes at p, of which `left` belong to the row; p is 16-byte aligned and nothing behind the row is touched
-__device__ __forceinline__ uint4 load_codes16(const uint8_t* __restrict__ p, int left) {
+__device__ __forceinline__ uint4 load_codes16(const uint8_t* p, int left) {
   if (left >= 16) return *reinterpret_cast<const uint4*>(p);
   uint32_t w[4] = {0, 0, 0, 0};
   for (int i = 0; i < left; ++i) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
@@ -54,7 +54,7 @@ __device__ __forceinline__ float few_row(uint32_t word[8], const FewArgs& g, uin
     const uint8_t* p = reinterpret_cast<const uint8_t*>(g.x) + row * g.x_pitch + col;
     const uint4 lo = load_codes16(p, (int)g.k - (int)col), hi = load_codes16(p + 16, (int)g.k - (int)col - 16);
     word[0] = lo.x; word[1] = lo.y; word[2] = lo.z; word[3] = lo.w; word[4] = hi.x; word[5] = hi.y; word[6] = hi.z; word[7] = hi.w;
-    return __ldg(g.a_scale + row * g.a_scale_row + kb * g.a_scale_block);
+    return g.a_scale[row * g.a_scale_row + kb * g.a_scale_block];
   } else {
     float v[32];
     float amax = amax_floor();
@@ -114,7 +114,7 @@ netra_dense_fp8_few_sm100(const FewArgs g) {
       if (kb >= blocks) break;
       const uint32_t lo[8] = {a[h][0].x, a[h][0].y, a[h][0].z, a[h][0].w, a[h][1].x, a[h][1].y, a[h][1].z, a[h][1].w};
       const uint32_t hi[8] = {a[h][2].x, a[h][2].y, a[h][2].z, a[h][2].w, a[h][3].x, a[h][3].y, a[h][3].z, a[h][3].w};
-      const float sw = __ldg(ws + kb);
+      const float sw = ws[kb];
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         uint32_t b[8];

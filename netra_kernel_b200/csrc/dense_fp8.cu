@@ -1,6 +1,6 @@
 // The dense block-scaled FP8 linear map, the operation the compiler's dense contract names
 // (compiler/netra_compiler/contracts.py:175-284): E4M3 codes with one FP32 scale per row and 128 columns on the left, per
-// 128 x 128 block on the right, FP32 accumulation, K-blocks ascending.
+// 128 x 128 block on the right, FP32 accumulation.
 //
 //   quantise   s[m,b] = max(amax |x[m, block b]|, 1e-10) * fl(1/448),  a = e4m3_rne_sat(x * fl(1/s))      (the layer's quantiser)
 //   product    y[m,n] = sum_b  sa[m,b] * sw[n/128,b] * sum_{k in b} a[m,k] w[n,k]
@@ -30,7 +30,8 @@ __device__ __forceinline__ void dense_store(void* p, uint32_t dtype, size_t i, f
 // The kernels here are launched while the kernel before them on the stream may still be running (programmatic dependent
 // launch): their launch, and the set-up of barriers and TMEM, overlap its end.  Every access to global memory comes after
 // begin_grid(), which waits until that kernel has completed and its writes are visible - stream order, as for any launch - and
-// lets the next such launch come as early.
+// lets the next such launch come as early.  Inputs may therefore be written while the grid already exists: no pointer here is
+// declared __restrict__ and nothing is read through the non-coherent path, whose data may not change in a kernel's lifetime.
 __device__ __forceinline__ void begin_grid() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -72,8 +73,8 @@ __device__ __forceinline__ void dense_load8(float v[8], const T* p) {
 
 template <typename T, bool kVector, int kRows>
 __global__ void __launch_bounds__(256)
-netra_dense_quantize_rows_sm100(const T* __restrict__ x, uint64_t x_pitch, uint8_t* __restrict__ codes, uint64_t codes_pitch,
-                                float* __restrict__ scale, uint64_t scale_row, uint64_t scale_block, uint32_t m, uint32_t k) {
+netra_dense_quantize_rows_sm100(const T* x, uint64_t x_pitch, uint8_t* codes, uint64_t codes_pitch,
+                                float* scale, uint64_t scale_row, uint64_t scale_block, uint32_t m, uint32_t k) {
   begin_grid();
   const uint32_t blocks = (k + kBlock - 1) / kBlock;
   const uint32_t item = (blockIdx.x * 256u + threadIdx.x) >> 4;
@@ -426,7 +427,7 @@ netra_dense_fp8_matmul_sm100(const __grid_constant__ CUtensorMap tm_a, const __g
       T* to = reinterpret_cast<T*>(g.out) + (uint64_t)first * g.out_pitch + col0 + lane;
       for (uint32_t r0 = warp; r0 < count; r0 += kRowsAtOnce * kWarps) {
         float v[kRowsAtOnce][kPerLane];
-        const float* p = parts + (size_t)r0 * C::kOutPitch + lane;     // rows past the share are summed in place and not stored
+        const float* p = parts + (size_t)r0 * C::kOutPitch + lane;
 #pragma unroll
         for (int i = 0; i < kRowsAtOnce; ++i)
 #pragma unroll

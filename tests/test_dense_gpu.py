@@ -311,6 +311,38 @@ def test_streams_and_captured_graphs():
     dense.check_status()
 
 
+@pytest.mark.parametrize("m", [3, 12, 20, 32, 200, 2600])
+def test_chains_of_dependent_calls(m):
+    """Each call reads what the one before it wrote, into memory that the allocator hands around, with nothing between them: the
+    kernels start before their predecessors end and must not see what the memory held earlier."""
+    n, depth = 512, 24
+    w, ws = make_weight(n, n, 13)
+    ws = ws / ws.mean() * 0.02
+    xs = [torch.randn(m, n, device="cuda", dtype=torch.bfloat16, generator=torch.Generator(device="cuda").manual_seed(i)) for i in range(4)]
+
+    def chain(x, wait):
+        for _ in range(depth):
+            x = dense.fp8_linear(x, w, ws)
+            if wait:
+                torch.cuda.synchronize()
+        return x
+
+    want = [chain(x, True) for x in xs]
+    for _ in range(20):
+        for x, y in zip(xs, want):
+            assert torch.equal(chain(x, False), y)
+    static, graph = xs[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(static, False)
+    for _ in range(5):
+        for x, y in zip(xs, want):
+            static.copy_(x)
+            graph.replay()
+            assert torch.equal(out, y)
+    assert bool(torch.isfinite(want[0]).all()) and bool((want[0] != 0).any())
+    dense.check_status()
+
+
 def test_capture_beside_a_living_eager_graph_of_the_leaf_is_refused():
     """torch itself cannot capture this backward pass; the call says so while the capture can still be ended."""
     w, ws = make_weight(64, 128, 1)
