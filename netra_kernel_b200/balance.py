@@ -36,3 +36,8 @@ def balance_loss(logits: torch.Tensor, counts: torch.Tensor, token_mask: Optiona
     loss is 0.  A masked expert (logit -inf, or the type's lowest value) has probability 0; a row whose logits are all -inf
     counts as a token and contributes 0.  NaN and +inf in a counted row give NaN."""
     return _ext.balance_loss(logits, counts, token_mask)
+
+
+def balance_loss_grad(upstream: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``upstream`` (FP32 scalar tensor) times the gradient of ``balance_loss`` with respect to logits, without autograd."""
+    return _ext.balance_loss_grad(upstream, logits, counts, token_mask)

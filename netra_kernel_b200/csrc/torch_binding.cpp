@@ -217,6 +217,19 @@ std::tuple<Tensor, Tensor> balance_forward(const Tensor& z, const Tensor& counts
   return {loss, scale};
 }
 
+Tensor balance_backward(const Tensor& z, const Tensor& counts, const uint8_t* mask, const Tensor& scale, const Tensor& upstream) {
+  const int64_t tokens = z.size(0), experts = z.size(1);
+  Tensor grad = at::empty({tokens, experts}, z.options());
+  if (tokens > 0) {
+    const c10::cuda::CUDAGuard guard(z.device());
+    check_rc(netra_balance_loss_grad_launch(grad.data_ptr(), experts, z.const_data_ptr(), element_code(z.scalar_type()), pitch_of(z),
+                                            counts.const_data_ptr<int32_t>(), mask, scale.const_data_ptr<float>(), upstream.const_data_ptr<float>(),
+                                            (uint64_t)tokens, (uint32_t)experts, stream_of(z)),
+             "balance_loss_grad_launch");
+  }
+  return grad;
+}
+
 struct BalanceFunction : torch::autograd::Function<BalanceFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
     const Tensor z = as_rows(logits, "logits");
@@ -226,30 +239,34 @@ struct BalanceFunction : torch::autograd::Function<BalanceFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &z = saved[0], &counts = saved[1], &mask = saved[2], &scale = saved[3];
-    const int64_t tokens = z.size(0), experts = z.size(1);
-    Tensor grad = at::empty({tokens, experts}, z.options());
-    if (tokens > 0) {
-      const c10::cuda::CUDAGuard guard(z.device());
-      check_rc(netra_balance_loss_grad_launch(grad.data_ptr(), experts, z.const_data_ptr(), element_code(z.scalar_type()), pitch_of(z),
-                                              counts.const_data_ptr<int32_t>(),
-                                              mask.defined() ? reinterpret_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr,
-                                              scale.const_data_ptr<float>(), grads[0].const_data_ptr<float>(), (uint64_t)tokens, (uint32_t)experts,
-                                              stream_of(z)),
-               "balance_loss_grad_launch");
-    }
+    const Tensor& mask = saved[2];
+    const Tensor grad = balance_backward(saved[0], saved[1], mask.defined() ? reinterpret_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr,
+                                         saved[3], grads[0]);
     return {once_differentiable(grad, grads[0]), Tensor(), Tensor()};
   }
 };
 
-Tensor balance_loss(const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
+const uint8_t* check_balance(const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && is_activation(logits.scalar_type()),
                     "logits must be a BF16, FP16 or FP32 CUDA matrix [tokens, experts]");
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, "experts must be 1..", kMaxExperts);
   TORCH_CHECK_VALUE(counts.scalar_type() == at::kInt && counts.device() == logits.device() && counts.dim() == 1 && counts.size(0) == experts &&
                         counts.is_contiguous(), "counts must be a contiguous int32 [experts] tensor on the same device");
-  const uint8_t* mask = mask_of(token_mask, tokens, logits.device());
+  return mask_of(token_mask, tokens, logits.device());
+}
+
+// the gradient alone (a traced graph's backward pass): the loss is computed again for its scale
+Tensor balance_loss_grad(const Tensor& upstream, const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
+  const uint8_t* mask = check_balance(logits, counts, token_mask);
+  TORCH_CHECK_VALUE(upstream.scalar_type() == at::kFloat && upstream.numel() == 1 && upstream.device() == logits.device(),
+                    "upstream must be an FP32 scalar on the same device");
+  const Tensor z = as_rows(logits.detach(), "logits");
+  return balance_backward(z, counts, mask, std::get<1>(balance_forward(z, counts, mask)), upstream);
+}
+
+Tensor balance_loss(const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
+  const uint8_t* mask = check_balance(logits, counts, token_mask);
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
     check_capture(logits);
     return BalanceFunction::apply(logits, counts, token_mask);
@@ -266,5 +283,6 @@ PYBIND11_MODULE(_netra_torch, m) {
   m.def("block_scaled_matmul", torch::wrap_pybind_function_no_gil(block_scaled_matmul));
   m.def("fp8_linear", torch::wrap_pybind_function_no_gil(fp8_linear));
   m.def("expert_counts", torch::wrap_pybind_function_no_gil(expert_counts));
+  m.def("balance_loss_grad", torch::wrap_pybind_function_no_gil(balance_loss_grad));
   m.def("balance_loss", torch::wrap_pybind_function_no_gil(balance_loss));
 }

@@ -9,6 +9,10 @@ A handle is a small integer naming a live layer object of this process; ``releas
 Both ops run on torch's current stream through ``libnetra_sm100.so`` and have fake (meta) kernels, so
 they can sit inside traced graphs; there is no CPU implementation.
 
+    y = torch.ops.netra.fp8_linear(x, weight, weight_scale)                    # dense.fp8_linear, with its gradient
+    counts = torch.ops.netra.expert_counts(topk_ids, 256, token_mask)          # balance.expert_counts
+    loss = torch.ops.netra.balance_loss(logits, counts, token_mask)            # balance.balance_loss, with its gradient
+
 Bring-up modes (the role of the reference's ``SGLANG_NETRA_ENGINE_MODE`` shadow / compare modes,
 ``docs/compiler/validation.md:187-193``), chosen by the environment variable ``NETRA_ENGINE_MODE`` when a layer is
 registered with its row-major weights (``register_layer(layer, shadow_weights=...)``):
@@ -21,6 +25,7 @@ from __future__ import annotations
 import torch
 
 import os
+from typing import Optional
 
 _layers: dict[int, object] = {}
 _shadow: dict[int, tuple] = {}
@@ -118,3 +123,87 @@ def moe_apply(hidden: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.
 @moe_apply.register_fake
 def _(hidden: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor, handle: int) -> torch.Tensor:
     return torch.empty_like(hidden)
+
+
+# The operators beside the layer (dense.py, balance.py) by name, for traced graphs.  Eager callers use the modules, which cost less
+# per call.
+@torch.library.custom_op("netra::fp8_linear", mutates_args=(), device_types="cuda")
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
+    from . import dense
+    return dense.fp8_linear(x, weight, weight_scale)
+
+
+@fp8_linear.register_fake
+def _(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+@torch.library.custom_op("netra::fp8_linear_input_grad", mutates_args=(), device_types="cuda")
+def fp8_linear_input_grad(grad: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
+    from . import dense
+    codes, scale = dense.quantize_rows(grad)
+    out = dense.block_scaled_matmul(codes, scale, weight, weight_scale, transpose_weight=True, out_dtype=grad.dtype)
+    return out.view(*grad.shape[:-1], weight.shape[1])
+
+
+@fp8_linear_input_grad.register_fake
+def _(grad: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
+    return grad.new_empty((*grad.shape[:-1], weight.shape[1]))
+
+
+def _keep_weight(ctx, inputs, output) -> None:
+    ctx.save_for_backward(*inputs[1:])
+
+
+def _linear_backward(ctx, grad):
+    return torch.ops.netra.fp8_linear_input_grad(grad, *ctx.saved_tensors), None, None
+
+
+fp8_linear.register_autograd(_linear_backward, setup_context=_keep_weight)
+
+
+@torch.library.custom_op("netra::expert_counts", mutates_args=(), device_types="cuda")
+def expert_counts(topk_ids: torch.Tensor, num_experts: int, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    from . import balance
+    return balance.expert_counts(topk_ids, num_experts, token_mask)
+
+
+@expert_counts.register_fake
+def _(topk_ids: torch.Tensor, num_experts: int, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return topk_ids.new_empty((num_experts,), dtype=torch.int32)
+
+
+@torch.library.custom_op("netra::balance_loss", mutates_args=(), device_types="cuda")
+def balance_loss(logits: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    from . import balance
+    return balance.balance_loss(logits, counts, token_mask)
+
+
+@balance_loss.register_fake
+def _(logits: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return logits.new_empty((), dtype=torch.float32)
+
+
+@torch.library.custom_op("netra::balance_loss_grad", mutates_args=(), device_types="cuda")
+def balance_loss_grad(upstream: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor,
+                      token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    from . import balance
+    return balance.balance_loss_grad(upstream, logits, counts, token_mask)
+
+
+@balance_loss_grad.register_fake
+def _(upstream: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return logits.new_empty(logits.shape)
+
+
+def _keep_routing(ctx, inputs, output) -> None:
+    logits, counts, ctx.has_mask = inputs[0], inputs[1], inputs[2] is not None
+    ctx.save_for_backward(logits, counts, *([inputs[2]] if ctx.has_mask else []))
+
+
+def _balance_backward(ctx, upstream):
+    logits, counts, *mask = ctx.saved_tensors
+    return torch.ops.netra.balance_loss_grad(upstream, logits, counts, mask[0] if ctx.has_mask else None), None, None
+
+
+balance_loss.register_autograd(_balance_backward, setup_context=_keep_routing)

@@ -225,6 +225,26 @@ def test_counts_of_the_layers_own_routing():
     layer.close()
 
 
+def test_operators_by_name_are_the_modules():
+    from netra_kernel_b200 import dense, torch_ops  # noqa: F401
+    g = torch.Generator().manual_seed(8)
+    z = torch.randn(70, 64, generator=g).cuda().requires_grad_()
+    ids = z.detach().topk(4, dim=1).indices
+    for mask in (None, (torch.rand(70, generator=g) < 0.5).cuda()):
+        counts = torch.ops.netra.expert_counts(ids, 64, mask)
+        assert torch.equal(counts, balance.expert_counts(ids, 64, mask))
+        loss = torch.ops.netra.balance_loss(z, counts, mask)
+        (dz,) = torch.autograd.grad(loss * 3, z)
+        want = balance.balance_loss(z, counts, mask)
+        assert torch.equal(loss, want) and torch.equal(dz, torch.autograd.grad(want * 3, z)[0])
+    w = (torch.randn(96, 64, generator=g) * 50).to(torch.float8_e4m3fn).cuda()
+    ws = torch.full((1, 1), 0.01, device="cuda")
+    x = z.detach().view(2, 35, 64).requires_grad_()
+    dy = torch.randn(2, 35, 96, generator=g).cuda()
+    y, want = torch.ops.netra.fp8_linear(x, w, ws), dense.fp8_linear(x, w, ws)
+    assert torch.equal(y, want) and torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(want, x, dy)[0])
+
+
 def test_refusals():
     z = torch.zeros(4, 16, device="cuda")
     counts = torch.ones(16, dtype=torch.int32, device="cuda")
@@ -235,6 +255,7 @@ def test_refusals():
         (lambda: balance.balance_loss(z, counts.long()), "counts"), (lambda: balance.balance_loss(z, counts[:15]), "counts"),
         (lambda: balance.balance_loss(z, counts.cpu()), "counts"), (lambda: balance.balance_loss(z, counts, mask[:3]), "token_mask"),
         (lambda: balance.balance_loss(z, counts, mask.float()), "token_mask"), (lambda: balance.balance_loss(z, counts, mask.cpu()), "token_mask"),
+        (lambda: balance.balance_loss_grad(mask.float(), z, counts), "upstream"), (lambda: balance.balance_loss_grad(z[0, 0], z, counts.long()), "counts"),
         (lambda: balance.expert_counts(z, 16), "topk_ids"), (lambda: balance.expert_counts(z.int()[0], 16), "topk_ids"),
         (lambda: balance.expert_counts(z.int(), 0), "num_experts"), (lambda: balance.expert_counts(z.int(), 1025), "num_experts"),
         (lambda: balance.expert_counts(z.int(), 16, mask[:2]), "token_mask"),

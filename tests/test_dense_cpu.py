@@ -75,3 +75,22 @@ def test_c_entries_refuse_before_any_launch():
     for kw, why in [(dict(g=None), "null"), (dict(s=None), "null"), (dict(u=None), "null"), (dict(gp=8), "pitch"), (dict(g=odd), "aligned")]:
         assert grad(**kw) == -1 and why in err(), kw
     assert isinstance(ctypes.c_uint64(size).value, int)
+
+
+def test_operators_by_name_trace_without_a_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from netra_kernel_b200 import torch_ops  # noqa: F401  (registers the operators)
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 256, dtype=torch.bfloat16, device="cuda")
+        w = torch.empty(300, 256, dtype=torch.float8_e4m3fn, device="cuda")
+        s = torch.empty(3, 2, device="cuda")
+        y = torch.ops.netra.fp8_linear(x, w, s)
+        assert y.shape == (2, 5, 300) and y.dtype == torch.bfloat16
+        dx = torch.ops.netra.fp8_linear_input_grad(y, w, s)
+        assert dx.shape == x.shape and dx.dtype == x.dtype
+        counts = torch.ops.netra.expert_counts(torch.empty(7, 8, dtype=torch.int32, device="cuda"), 60)
+        assert counts.shape == (60,) and counts.dtype == torch.int32
+        z = torch.empty(7, 60, device="cuda")
+        loss = torch.ops.netra.balance_loss(z, counts)
+        dz = torch.ops.netra.balance_loss_grad(loss, z, counts)
+        assert loss.shape == () and loss.dtype == torch.float32 and dz.shape == z.shape
