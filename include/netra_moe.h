@@ -481,8 +481,9 @@ int netra_expert_counts_launch(int32_t* counts_i32, const void* ids, uint32_t id
 /* With f = counts / sum counts, p_t = softmax(logits_t) and n counted tokens:
  *   loss = experts / n * sum_t sum_e f_e p_te          grad_te = upstream * experts / n * p_te * (f_e - sum_j f_j p_tj)
  * scale_f32 receives experts / n, which the gradient reads.  No counted token, or no count: 0.  A row without a finite logit counts as a token and contributes 0; rows not counted are not read and get
- * a zero gradient.  The workspace (16-byte aligned) is free again when the call's work is done on the stream. */
-uint64_t netra_balance_loss_workspace_bytes(void);
+ * a zero gradient.  The workspace (16-byte aligned; none for small calls: 0 bytes) is free again when the call's work is done
+ * on the stream. */
+uint64_t netra_balance_loss_workspace_bytes(uint64_t tokens, uint32_t experts);
 int netra_balance_loss_launch(float* loss_f32, float* scale_f32, const void* logits, uint32_t dtype, uint64_t pitch,
                               const int32_t* counts_i32, const uint8_t* token_mask, void* workspace,
                               uint64_t workspace_bytes, uint64_t tokens, uint32_t experts, cudaStream_t stream);

@@ -114,7 +114,7 @@ SIGNATURES = {
                                               c_u32, c_u32, c_void_p, c_u64, c_void_p]),
     "netra_dense_status": (c_int, [ctypes.POINTER(c_u32 * 4)]),
     "netra_expert_counts_launch": (c_int, [c_void_p, c_void_p, c_u32, c_u64, c_void_p, c_u64, c_u32, c_u32, c_void_p]),
-    "netra_balance_loss_workspace_bytes": (c_u64, []),
+    "netra_balance_loss_workspace_bytes": (c_u64, [c_u64, c_u32]),
     "netra_balance_loss_launch": (c_int, [c_void_p, c_void_p, c_void_p, c_u32, c_u64, c_void_p, c_void_p, c_void_p, c_u64, c_u64, c_u32, c_void_p]),
     "netra_balance_loss_grad_launch": (c_int, [c_void_p, c_u64, c_void_p, c_u32, c_u64, c_void_p, c_void_p, c_void_p, c_void_p, c_u64,
                                                c_u32, c_void_p]),

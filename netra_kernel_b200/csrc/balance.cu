@@ -317,6 +317,8 @@ int balance_check(const char* what, const void* z, uint32_t dtype, uint64_t pitc
   return 0;
 }
 
+bool balance_one_cluster(uint64_t tokens, uint32_t experts) { return tokens <= kLossClusterTokens && experts <= 512; }
+
 uint32_t balance_blocks(uint64_t tokens) {
   const uint64_t b = (tokens + kBalThreads / 32 - 1) / (kBalThreads / 32);
   return (uint32_t)(b < kBalMaxBlocks ? b : kBalMaxBlocks);
@@ -368,17 +370,20 @@ int netra_expert_counts_launch(int32_t* counts_i32, const void* ids, uint32_t id
                                    id_pitch, token_mask, counts_i32, tokens, slots, experts));
 }
 
-uint64_t netra_balance_loss_workspace_bytes(void) { return 16 + kBalMaxBlocks * sizeof(BalPartial); }
+uint64_t netra_balance_loss_workspace_bytes(uint64_t tokens, uint32_t experts) {
+  return balance_one_cluster(tokens, experts) ? 0 : 16 + kBalMaxBlocks * sizeof(BalPartial);
+}
 
 int netra_balance_loss_launch(float* loss_f32, float* scale_f32, const void* logits, uint32_t dtype, uint64_t pitch, const int32_t* counts_i32,
                               const uint8_t* token_mask, void* workspace, uint64_t workspace_bytes, uint64_t tokens, uint32_t experts,
                               cudaStream_t stream) {
   if (int rc = balance_check("balance_loss", logits, dtype, pitch, counts_i32, tokens, experts)) return rc;
-  if (!loss_f32 || !scale_f32 || !workspace) return fail("balance_loss: null pointer");
-  if (workspace_bytes < netra_balance_loss_workspace_bytes() || (uintptr_t)workspace % 16) return fail("balance_loss: workspace too small or not 16-byte aligned");
+  if (!loss_f32 || !scale_f32) return fail("balance_loss: null pointer");
+  const uint64_t needed = netra_balance_loss_workspace_bytes(tokens, experts);
+  if (needed > 0 && (!workspace || workspace_bytes < needed || (uintptr_t)workspace % 16)) return fail("balance_loss: workspace missing, too small or not 16-byte aligned");
   const bool aligned = balance_aligned(logits, pitch, dtype, experts);
   cudaError_t launch = cudaSuccess;
-  if (tokens <= kLossClusterTokens && experts <= 512) {
+  if (needed == 0) {
     balance_shape(dtype, aligned, experts, [&](auto element, auto access, auto per) {
       using T = decltype(element);
       if constexpr (decltype(per)::value <= 16)

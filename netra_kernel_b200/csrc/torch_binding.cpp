@@ -208,10 +208,10 @@ std::tuple<Tensor, Tensor> balance_forward(const Tensor& z, const Tensor& counts
   if (tokens == 0) return {at::zeros({}, options), Tensor()};
   Tensor loss = at::empty({}, options), scale = at::empty({}, options);
   const c10::cuda::CUDAGuard guard(z.device());
-  const uint64_t bytes = netra_balance_loss_workspace_bytes();
-  const Tensor workspace = at::empty({(int64_t)bytes}, z.options().dtype(at::kByte));
+  const uint64_t bytes = netra_balance_loss_workspace_bytes((uint64_t)tokens, (uint32_t)experts);
+  const Tensor workspace = bytes > 0 ? at::empty({(int64_t)bytes}, z.options().dtype(at::kByte)) : Tensor();
   check_rc(netra_balance_loss_launch(loss.data_ptr<float>(), scale.data_ptr<float>(), z.const_data_ptr(), element_code(z.scalar_type()), pitch_of(z),
-                                     counts.const_data_ptr<int32_t>(), mask, workspace.data_ptr(), bytes, (uint64_t)tokens, (uint32_t)experts,
+                                     counts.const_data_ptr<int32_t>(), mask, bytes > 0 ? workspace.data_ptr() : nullptr, bytes, (uint64_t)tokens, (uint32_t)experts,
                                      stream_of(z)),
            "balance_loss_launch");
   return {loss, scale};

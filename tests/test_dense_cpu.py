@@ -65,10 +65,11 @@ def test_c_entries_refuse_before_any_launch():
     for kw, why in [(dict(c=None), "null"), (dict(ids=None), "null"), (dict(b=2), "bytes"), (dict(pitch=7), "pitch"), (dict(e=0), "1024"),
                     (dict(e=1025), "1024"), (dict(t=1 << 30), "2^31"), (dict(ids=4098), "aligned")]:
         assert cnt(**kw) == -1 and why in err(), kw
-    size = lib.netra_balance_loss_workspace_bytes()
-    loss = lambda l=p, sc=p, z=p, dt=0, pitch=16, c=p, w=p, n=size, t=2, e=16: lib.netra_balance_loss_launch(l, sc, z, dt, pitch, c, None, w, n, t, e, None)   # noqa: E731
+    assert lib.netra_balance_loss_workspace_bytes(2, 16) == 0            # small calls need none
+    size = lib.netra_balance_loss_workspace_bytes(5000, 16)
+    loss = lambda l=p, sc=p, z=p, dt=0, pitch=16, c=p, w=p, n=size, t=5000, e=16: lib.netra_balance_loss_launch(l, sc, z, dt, pitch, c, None, w, n, t, e, None)   # noqa: E731
     for kw, why in [(dict(l=None), "null"), (dict(sc=None), "null"), (dict(z=None), "null"), (dict(c=None), "null"), (dict(dt=3), "type"),
-                    (dict(pitch=15), "pitch"), (dict(w=None), "null"), (dict(n=size - 1), "workspace"), (dict(w=p + 8), "workspace"),
+                    (dict(pitch=15), "pitch"), (dict(w=None), "workspace"), (dict(n=size - 1), "workspace"), (dict(w=p + 8), "workspace"),
                     (dict(t=0), "tokens"), (dict(e=0), "1024"), (dict(e=2000), "1024"), (dict(z=odd), "aligned")]:
         assert loss(**kw) == -1 and why in err(), kw
     grad = lambda g=p, gp=16, s=p, u=p: lib.netra_balance_loss_grad_launch(g, gp, p, 0, 16, p, None, s, u, 2, 16, None)                  # noqa: E731
