@@ -459,8 +459,11 @@ int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pi
 
 /* Both in one call: quantises the rows of x into the workspace and multiplies; out has x's type.  The workspace is 16-byte
  * aligned device memory of netra_dense_fp8_linear_workspace_bytes(m, reduction length) bytes, free again when the
- * call's work is done on the stream. */
+ * call's work is done on the stream.  netra_dense_fp8_linear_needs_workspace is 0 where the product quantises the rows
+ * itself (few rows on 16-byte boundaries); the workspace may then be NULL. */
 uint64_t netra_dense_fp8_linear_workspace_bytes(uint32_t m, uint32_t k);
+uint32_t netra_dense_fp8_linear_needs_workspace(const void* x, uint32_t dtype, uint64_t x_pitch, uint32_t transpose_w, uint32_t m,
+                                                uint32_t k);
 int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, uint32_t dtype, uint64_t x_pitch,
                                   const void* w_fp8, uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch,
                                   uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols, void* workspace,

@@ -110,6 +110,7 @@ SIGNATURES = {
     "netra_dense_fp8_matmul_launch": (c_int, [c_void_p, c_u32, c_u64, c_void_p, c_u64, c_void_p, c_u64, c_u64, c_void_p, c_u64, c_void_p,
                                               c_u64, c_u32, c_u32, c_u32, c_u32, c_void_p]),
     "netra_dense_fp8_linear_workspace_bytes": (c_u64, [c_u32, c_u32]),
+    "netra_dense_fp8_linear_needs_workspace": (c_u32, [c_void_p, c_u32, c_u64, c_u32, c_u32, c_u32]),
     "netra_dense_fp8_linear_launch": (c_int, [c_void_p, c_u64, c_void_p, c_u32, c_u64, c_void_p, c_u64, c_void_p, c_u64, c_u32, c_u32,
                                               c_u32, c_u32, c_void_p, c_u64, c_void_p]),
     "netra_dense_status": (c_int, [ctypes.POINTER(c_u32 * 4)]),

@@ -724,17 +724,19 @@ uint64_t netra_dense_fp8_linear_workspace_bytes(uint32_t m, uint32_t k) {
   return (uint64_t)m * blocks * (128 + 4);
 }
 
+uint32_t netra_dense_fp8_linear_needs_workspace(const void* x, uint32_t dtype, uint64_t x_pitch, uint32_t transpose_w, uint32_t m, uint32_t k) {
+  // Few rows: the product quantises them itself, if whole 16-byte accesses fit them.  Every CTA reads all of them, so FP32 rows
+  // pay up to four (4 x 4096 x 2048: 5.4 us against 5.9 us with the quantiser's launch, 8 rows 7.6 us against 6.0 us), 16-bit ones up
+  // to sixteen (5.8 us against 6.3 us).
+  return transpose_w || m > (dtype == kDenseF32 ? 4u : kFewMaxRows) || k % 8 != 0 || (uintptr_t)x % 16 != 0 ||
+         x_pitch * dense_element_bytes(dtype) % 16 != 0;
+}
+
 int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, uint32_t dtype, uint64_t x_pitch, const void* w_fp8,
                                   uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch, uint32_t transpose_w, uint32_t m,
                                   uint32_t w_rows, uint32_t w_cols, void* workspace, uint64_t workspace_bytes, cudaStream_t stream) {
   const uint32_t k = transpose_w ? w_rows : w_cols;
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < netra_dense_fp8_linear_workspace_bytes(m, k))
-    return fail("dense_fp8_linear: workspace missing, too small or not 16-byte aligned");
-  const uint64_t pitch = ((uint64_t)k + 127) / 128 * 128;
-  // Few rows: the product quantises them itself, if whole 16-byte accesses fit them.  Every CTA reads all of them, so FP32 rows
-  // pay up to four (4 x 4096 x 2048: 5.4 us against 5.9 us with the quantiser's launch, 8 rows 7.6 us against 6.0 us), 16-bit ones up
-  // to sixteen (5.8 us against 6.3 us).
-  if (!transpose_w && m <= (dtype == kDenseF32 ? 4u : kFewMaxRows) && k % 8 == 0 && (uintptr_t)x % 16 == 0 && x_pitch * dense_element_bytes(dtype) % 16 == 0) {
+  if (!netra_dense_fp8_linear_needs_workspace(x, dtype, x_pitch, transpose_w, m, k)) {
     if (int rc = check_quantize_operands(x, dtype, x_pitch, m, k)) return rc;
     if (int rc = check_matmul_operands(out, dtype, out_pitch, w_fp8, w_pitch, w_scale_f32, w_scale_pitch, transpose_w, m, w_rows, w_cols)) return rc;
     int sms = 0;
@@ -743,6 +745,9 @@ int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, 
     const FewArgs f = {x, x_pitch, nullptr, 0, 0, (const uint8_t*)w_fp8, w_pitch, w_scale_f32, w_scale_pitch, out, out_pitch, dtype, m, w_rows, k};
     return launch_few(f, dtype, sms, stream);
   }
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < netra_dense_fp8_linear_workspace_bytes(m, k))
+    return fail("dense_fp8_linear: workspace missing, too small or not 16-byte aligned");
+  const uint64_t pitch = ((uint64_t)k + 127) / 128 * 128;
   uint8_t* codes = (uint8_t*)workspace;
   float* scale = (float*)(codes + (uint64_t)m * pitch);
   if (int rc = netra_dense_quantize_rows_launch(codes, pitch, scale, 1, m, x, dtype, x_pitch, m, k, stream)) return rc;

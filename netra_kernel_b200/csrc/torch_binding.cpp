@@ -122,11 +122,15 @@ Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool trans
   Tensor out = at::empty({m, n}, x.options());
   if (m > 0) {
     const c10::cuda::CUDAGuard guard(x.device());
-    const uint64_t bytes = netra_dense_fp8_linear_workspace_bytes((uint32_t)m, (uint32_t)k);
-    const Tensor workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    uint64_t bytes = 0;
+    Tensor workspace;
+    if (netra_dense_fp8_linear_needs_workspace(x.const_data_ptr(), element_code(x.scalar_type()), pitch_of(x), transposed, (uint32_t)m, (uint32_t)k)) {
+      bytes = netra_dense_fp8_linear_workspace_bytes((uint32_t)m, (uint32_t)k);
+      workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    }
     check_rc(netra_dense_fp8_linear_launch(out.data_ptr(), n, x.const_data_ptr(), element_code(x.scalar_type()), pitch_of(x), w.const_data_ptr(),
                                            code_pitch_of(w), ws.const_data_ptr<float>(), pitch_of(ws), transposed, (uint32_t)m, (uint32_t)w.size(0),
-                                           (uint32_t)w.size(1), workspace.data_ptr(), bytes, stream_of(x)),
+                                           (uint32_t)w.size(1), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(x)),
              "dense_fp8_linear_launch");
   }
   if (input.dim() == 2) return out;

@@ -60,6 +60,10 @@ def test_c_entries_refuse_before_any_launch():
     lin = lambda ws=p, size=size: lib.netra_dense_fp8_linear_launch(p, 64, p, 0, 130, p, 144, p, 2, 0, 3, 64, 130, ws, size, None)      # noqa: E731
     for kw in (dict(ws=None), dict(ws=p + 8), dict(size=size - 1)):
         assert lin(**kw) == -1 and "workspace" in err(), kw
+    needs = lambda x=p, dt=0, xp=128, tr=0, m=16, k=128: lib.netra_dense_fp8_linear_needs_workspace(x, dt, xp, tr, m, k)               # noqa: E731
+    assert needs() == 0 and needs(m=1, dt=2) == 0
+    for kw in (dict(m=17), dict(tr=1), dict(k=130), dict(x=p + 2), dict(xp=130), dict(dt=2)):
+        assert needs(**kw) == 1, kw
     assert lib.netra_dense_status(None) == -1
     cnt = lambda c=p, ids=p, b=4, pitch=8, t=2, s=8, e=256: lib.netra_expert_counts_launch(c, ids, b, pitch, None, t, s, e, None)       # noqa: E731
     for kw, why in [(dict(c=None), "null"), (dict(ids=None), "null"), (dict(b=2), "bytes"), (dict(pitch=7), "pitch"), (dict(e=0), "1024"),
