@@ -82,7 +82,9 @@ struct BalLane {
       const uint32_t e = expert(i, lane);
       if (kAligned && e < experts) {
         if constexpr (kVec == 8) {
-          dense_load8(v + i, row + e);
+          Eight<T> x8;
+          x8.load(row + e);
+          x8.values(v + i);
         } else {
           const float4 f = *reinterpret_cast<const float4*>(row + e);
           v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;

@@ -56,25 +56,26 @@ __device__ __forceinline__ float few_row(uint32_t word[8], const FewArgs& g, uin
     word[0] = lo.x; word[1] = lo.y; word[2] = lo.z; word[3] = lo.w; word[4] = hi.x; word[5] = hi.y; word[6] = hi.z; word[7] = hi.w;
     return g.a_scale[row * g.a_scale_row + kb * g.a_scale_block];
   } else {
-    float v[32];
+    Eight<T> x8[4];
     float amax = amax_floor();
     const T* p = reinterpret_cast<const T*>(g.x) + row * g.x_pitch + col;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      if (row < g.m && col + 8 * c < g.k) {         // the host passes widths that are multiples of eight
-        dense_load8(v + 8 * c, p + 8 * c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * c + j] = 0.0f;
-      }
+      if (row < g.m && col + 8 * c < g.k) x8[c].load(p + 8 * c);         // the host passes widths that are multiples of eight
+      else x8[c].clear();
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) amax = fmaxf(amax, fabsf(v[j]));
+    for (int c = 0; c < 4; ++c) amax = fmaxf(amax, x8[c].amax());
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const float s = amax * inv448(), inv = 1.0f / s;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) word[j] = f32x4_to_e4m3x4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+    for (int c = 0; c < 4; ++c) {
+      float v[8];
+      x8[c].values(v);
+      word[2 * c] = f32x4_to_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+      word[2 * c + 1] = f32x4_to_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    }
     return s;
   }
 }
