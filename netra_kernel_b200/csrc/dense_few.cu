@@ -10,6 +10,7 @@
 //   * Source rows of BF16 / FP16 / FP32 are quantised by the warp that multiplies them (each warp sees its own K-blocks of all
 //     rows: no block of a row is quantised twice by one CTA), which saves the quantiser's launch.
 // Per K-block the raw FP32 sums are promoted as acc = fma(part, sa * sw, acc); the warps' sums are added in warp order.
+// Measured (BF16 rows, quantising included, in a graph): 1 x 2048 x 4096 3.7-3.8 us, 8 x 4096 x 2048 4.1-4.2 us, 12 x 4096 x 2048 5.7 us.
 namespace netra {
 
 constexpr int kFewRows = 16;            // weight rows of a CTA

@@ -80,8 +80,8 @@ struct Eight {
       raw[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
   }
-  // In FP32: maxima of packed 16-bit pairs gained 7 % on the largest quantiser calls (16384 x 2048 BF16: 18.3 -> 16.9 us), but cost the
-  // latency-bound ones more (1024 x 4096: 2.8 -> 3.6 us, the few-row product at 8 x 4096 x 2048: 4.3 -> 5.6 us).
+  // In FP32: maxima of packed 16-bit pairs gained 7 % on the largest quantiser calls (16384 x 2048 BF16: 18.2 -> 16.9 us), but cost the
+  // latency-bound ones more (1024 x 4096: 2.9 -> 3.6 us, the few-row product at 8 x 4096 x 2048: 4.4 -> 5.6 us).
   __device__ __forceinline__ float amax() const {
     float v[8];
     values(v);
