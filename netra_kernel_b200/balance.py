@@ -34,7 +34,8 @@ def balance_loss(logits: torch.Tensor, counts: torch.Tensor, token_mask: Optiona
 
     Tokens that ``token_mask`` leaves out are not read and get a zero gradient; with no counted token, or no counts, the
     loss is 0.  A masked expert (logit -inf, or the type's lowest value) has probability 0; a row whose logits are all -inf
-    counts as a token and contributes 0.  NaN and +inf in a counted row give NaN."""
+    counts as a token and contributes 0.  NaN and +inf in a counted row give NaN.  The gradient cannot be differentiated again: a
+    second derivative raises RuntimeError."""
     return _ext.balance_loss(logits, counts, token_mask)
 
 

@@ -9,7 +9,6 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -139,12 +138,10 @@ Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool trans
   return out.view(shape);
 }
 
-// gradients of a backward pass that is itself being differentiated: an error once somebody asks for them
-Tensor once_differentiable(Tensor grad, const Tensor& upstream) {
-  if (!at::GradMode::is_enabled() || !upstream.requires_grad()) return grad;
-  auto error = std::make_shared<torch::autograd::DelayedError>("this gradient cannot be differentiated again", 1);
-  return (*error)({grad.detach().requires_grad_()})[0];
-}
+// The gradients have no derivatives of their own.  A backward pass that is itself being differentiated (create_graph) computes its
+// gradient through a node that hangs on everything the gradient depends on and raises once a second derivative reaches it; a
+// tensor without that node would count as a constant, and its terms would be missing from a sum without a word.
+[[noreturn]] variable_list refuse_second_derivative() { TORCH_CHECK(false, "this gradient cannot be differentiated again"); }
 
 // A leaf keeps its gradient node, with the stream it was made on, for as long as any graph of it lives.  If that was the default
 // stream, a backward pass captured on another one makes torch tie the two together, which CUDA forbids and which invalidates the
@@ -159,6 +156,11 @@ void check_capture(const Tensor& x) {
               "forward and backward pass of the same leaf, or capture with a fresh leaf");
 }
 
+struct LinearGradFunction : torch::autograd::Function<LinearGradFunction> {
+  static Tensor forward(AutogradContext*, const Tensor& dy, const Tensor& w, const Tensor& ws) { return linear(dy, w, ws, true); }
+  static variable_list backward(AutogradContext*, const variable_list&) { return refuse_second_derivative(); }
+};
+
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& ws) {
     ctx->save_for_backward({w, ws});
@@ -166,7 +168,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
-    return {once_differentiable(linear(grads[0].detach(), saved[0], saved[1], true), grads[0]), Tensor(), Tensor()};
+    const Tensor& dy = grads[0];
+    return {at::GradMode::is_enabled() ? LinearGradFunction::apply(dy, saved[0], saved[1]) : linear(dy, saved[0], saved[1], true), Tensor(), Tensor()};
   }
 };
 
@@ -209,7 +212,7 @@ Tensor expert_counts(const Tensor& topk_ids, int64_t experts, const std::optiona
 std::tuple<Tensor, Tensor> balance_forward(const Tensor& z, const Tensor& counts, const uint8_t* mask) {
   const int64_t tokens = z.size(0), experts = z.size(1);
   const auto options = z.options().dtype(at::kFloat);
-  if (tokens == 0) return {at::zeros({}, options), Tensor()};
+  if (tokens == 0) return {at::zeros({}, options), at::zeros({}, options)};
   Tensor loss = at::empty({}, options), scale = at::empty({}, options);
   const c10::cuda::CUDAGuard guard(z.device());
   const uint64_t bytes = netra_balance_loss_workspace_bytes((uint64_t)tokens, (uint32_t)experts);
@@ -234,19 +237,32 @@ Tensor balance_backward(const Tensor& z, const Tensor& counts, const uint8_t* ma
   return grad;
 }
 
+const uint8_t* saved_mask(const std::optional<Tensor>& mask) {
+  return mask.has_value() && mask->defined() ? reinterpret_cast<const uint8_t*>(mask->const_data_ptr()) : nullptr;
+}
+
+struct BalanceGradFunction : torch::autograd::Function<BalanceGradFunction> {
+  static Tensor forward(AutogradContext*, const Tensor& upstream, const Tensor& z, const Tensor& counts, const Tensor& scale,
+                        const std::optional<Tensor>& mask) {
+    return balance_backward(z, counts, saved_mask(mask), scale, upstream);
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) { return refuse_second_derivative(); }
+};
+
+// z: logits as rows the kernels can walk; a copy, where it is one, was made outside, so that z still hangs on them
 struct BalanceFunction : torch::autograd::Function<BalanceFunction> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
-    const Tensor z = as_rows(logits, "logits");
-    auto [loss, scale] = balance_forward(z, counts, mask_of(token_mask, z.size(0), z.device()));
-    ctx->save_for_backward({z, counts, token_mask.value_or(Tensor()), scale});
+  static Tensor forward(AutogradContext* ctx, const Tensor& z, const Tensor& counts, const std::optional<Tensor>& token_mask) {
+    auto [loss, scale] = balance_forward(z, counts, saved_mask(token_mask));
+    ctx->save_for_backward({z, counts, scale, token_mask.value_or(Tensor())});
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor& mask = saved[2];
-    const Tensor grad = balance_backward(saved[0], saved[1], mask.defined() ? reinterpret_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr,
-                                         saved[3], grads[0]);
-    return {once_differentiable(grad, grads[0]), Tensor(), Tensor()};
+    const Tensor &z = saved[0], &counts = saved[1], &scale = saved[2];
+    const auto mask = saved[3].defined() ? std::optional<Tensor>(saved[3]) : std::nullopt;
+    return {at::GradMode::is_enabled() ? BalanceGradFunction::apply(grads[0], z, counts, scale, mask)
+                                       : balance_backward(z, counts, saved_mask(mask), scale, grads[0]),
+            Tensor(), Tensor()};
   }
 };
 
@@ -273,7 +289,7 @@ Tensor balance_loss(const Tensor& logits, const Tensor& counts, const std::optio
   const uint8_t* mask = check_balance(logits, counts, token_mask);
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
     check_capture(logits);
-    return BalanceFunction::apply(logits, counts, token_mask);
+    return BalanceFunction::apply(as_rows(logits, "logits"), counts, token_mask);
   }
   return std::get<0>(balance_forward(as_rows(logits, "logits"), counts, mask));
 }

@@ -49,7 +49,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
     Differentiable with respect to x: the incoming gradient's rows are quantised the same way and multiplied by the weight as
     it is stored (``block_scaled_matmul(..., transpose_weight=True)``); the rounding of x to E4M3 passes gradients unchanged.
-    The weight is frozen."""
+    The weight is frozen.  The gradient cannot be differentiated again with respect to the incoming one: that raises RuntimeError."""
     return _ext.fp8_linear(x, weight, weight_scale)
 
 

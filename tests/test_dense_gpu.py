@@ -467,3 +467,38 @@ def test_router_fine_tuning_step():
     assert float((hidden.grad.cpu().double() - want_hidden).norm() / want_hidden.norm()) < 2.0 ** -4
     assert bool((hidden.grad[~mask] == 0).all())
     assert abi.load().netra_moe_last_error() is not None
+
+
+def test_second_derivatives_are_refused_in_every_call():
+    """The loss's gradient depends on the logits themselves, so whatever the upstream gradient is, nothing that holds it can be
+    differentiated again: neither back to all leaves nor to chosen ones, and not through a copy of strided logits."""
+    from netra_kernel_b200 import torch_ops  # noqa: F401
+    counts = torch.arange(16, dtype=torch.int32, device="cuda")
+    scale = torch.full((), 2.0, device="cuda")
+    for loss_of in (balance.balance_loss, torch.ops.netra.balance_loss):
+        for base, view in ((torch.randn(5, 16), lambda t: t), (torch.randn(16, 5), lambda t: t.t())):
+            for upstream in (None, scale, scale.clone().requires_grad_()):
+                z = base.cuda().requires_grad_()
+                loss = loss_of(view(z), counts)
+                (dz,) = torch.autograd.grad(loss, z, upstream, create_graph=True)
+                penalty = dz.pow(2).sum()
+                for again in (lambda: (loss + penalty).backward(retain_graph=True), lambda: torch.autograd.grad(loss + penalty, z, retain_graph=True),
+                              lambda: torch.autograd.grad(penalty, z, retain_graph=True)):
+                    with pytest.raises(RuntimeError):
+                        again()
+            with pytest.raises(RuntimeError):
+                torch.autograd.functional.hessian(lambda v: loss_of(view(v), counts), base.cuda())
+            loss = loss_of(view(z), counts)                            # a first derivative stays a plain tensor
+            (dz,) = torch.autograd.grad(loss, z)
+            assert not dz.requires_grad
+    w, ws = make_weight(32, 128, 1)
+    for linear in (dense.fp8_linear, torch.ops.netra.fp8_linear):
+        x = torch.randn(3, 128, device="cuda").requires_grad_()
+        dy = torch.ones(3, 32, device="cuda").requires_grad_()
+        y = linear(x, w, ws)
+        (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+        for again in (lambda: torch.autograd.grad(dx.sum() + dy.sum(), dy, retain_graph=True), lambda: (y.sum() + dx.pow(2).sum()).backward()):
+            with pytest.raises(RuntimeError):
+                again()
+        (dx,) = torch.autograd.grad(linear(x, w, ws), x, dy.detach(), create_graph=True)       # depends on nothing that is differentiated
+        assert torch.equal(dx, torch.autograd.grad(linear(x, w, ws), x, dy.detach())[0])
