@@ -7,7 +7,7 @@ With f = counts / sum counts and P_e the mean softmax probability of expert e ov
 ``loss = E * sum_e f_e * P_e``: 1 when both are even.  The counts carry no gradient; a data- or expert-parallel program adds
 up the ranks' counts before it calls ``balance_loss``.  Calls enqueue on torch's current stream of the operands' device and may
 be captured in a CUDA graph; results do not depend on the order in which blocks run.  There is no CPU implementation.
-Bad operands raise ValueError, failures of the C ABI RuntimeError.
+Bad operands raise ValueError, operands that carry a forward-mode tangent NotImplementedError, failures of the C ABI RuntimeError.
 """
 from __future__ import annotations
 

@@ -33,6 +33,11 @@ void check_rc(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (c
 
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// The kernels compute no tangents; an output without one would count as a constant in forward-mode differentiation.
+void refuse_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "forward-mode derivatives are not supported: an operand carries a tangent");
+}
+
 // x as a matrix whose rows the kernels can walk: unit column stride, rows that do not overlap
 Tensor as_rows(const Tensor& x, const char* what) {
   TORCH_CHECK_VALUE(x.is_cuda(), what, " must be a CUDA tensor");
@@ -58,12 +63,15 @@ void check_weight(const Tensor& w, const Tensor& s, const at::Device& device) {
   TORCH_CHECK_VALUE(s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == ceil_div(n, kBlockCols) && s.size(1) == ceil_div(k, kBlockCols),
                     "weight_scale must be float32 [ceil(N/128), ceil(K/128)]");
   TORCH_CHECK_VALUE((s.stride(1) == 1 || s.size(1) == 1) && (s.stride(0) >= s.size(1) || s.size(0) == 1), "weight_scale must be row-major");
+  refuse_tangent(w);
+  refuse_tangent(s);
   TORCH_CHECK_VALUE(!w.requires_grad() && !s.requires_grad(), "the FP8 weight is frozen: it cannot require a gradient");
 }
 
 void check_weight_on(const Tensor& w, const Tensor& s, const at::Device& device) { check_weight(w, s, device); }
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& input) {
+  refuse_tangent(input);
   const Tensor x = as_rows(input.detach(), "x");
   TORCH_CHECK_VALUE(x.size(0) <= kMaxSize && x.size(1) <= kMaxSize, "sizes must not exceed 2^26");
   const int64_t m = x.size(0), k = x.size(1), blocks = ceil_div(k, kBlockCols), pitch = blocks * kBlockCols;
@@ -86,6 +94,8 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
                            at::ScalarType out_dtype, const std::optional<Tensor>& out_given) {
   TORCH_CHECK_VALUE(a.is_cuda() && a.scalar_type() == at::kFloat8_e4m3fn && a.dim() == 2, "a must be a float8_e4m3fn CUDA matrix");
   check_weight(w, ws, a.device());
+  refuse_tangent(a);
+  refuse_tangent(a_scale);
   const int64_t m = a.size(0), k = w.size(transpose_weight ? 0 : 1), n = w.size(transpose_weight ? 1 : 0);
   check_sizes(m, w);
   TORCH_CHECK_VALUE(a.size(1) == k, "a has ", a.size(1), " columns, the weight reduces over ", k);
@@ -96,6 +106,7 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
   Tensor out;
   if (out_given.has_value()) {
     out = *out_given;
+    refuse_tangent(out);
     TORCH_CHECK_VALUE(out.device() == a.device() && is_activation(out.scalar_type()) && out.dim() == 2 && out.size(0) == m && out.size(1) == n &&
                           (out.stride(1) == 1 || n == 1) && (out.stride(0) >= n || m <= 1) && !out.requires_grad(),
                       "out must be a row-major [M, N] matrix of BF16, FP16 or FP32 on a's device");
@@ -115,6 +126,7 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
 }
 
 Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool transposed) {
+  refuse_tangent(input);
   const Tensor x = as_rows(input, "x");
   const int64_t m = x.size(0), k = w.size(transposed ? 0 : 1), n = w.size(transposed ? 1 : 0);
   check_sizes(m, w);
@@ -225,6 +237,7 @@ std::tuple<Tensor, Tensor> balance_forward(const Tensor& z, const Tensor& counts
 }
 
 Tensor balance_backward(const Tensor& z, const Tensor& counts, const uint8_t* mask, const Tensor& scale, const Tensor& upstream) {
+  refuse_tangent(upstream);
   const int64_t tokens = z.size(0), experts = z.size(1);
   Tensor grad = at::empty({tokens, experts}, z.options());
   if (tokens > 0) {
@@ -269,6 +282,7 @@ struct BalanceFunction : torch::autograd::Function<BalanceFunction> {
 const uint8_t* check_balance(const Tensor& logits, const Tensor& counts, const std::optional<Tensor>& token_mask) {
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && is_activation(logits.scalar_type()),
                     "logits must be a BF16, FP16 or FP32 CUDA matrix [tokens, experts]");
+  refuse_tangent(logits);
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, "experts must be 1..", kMaxExperts);
   TORCH_CHECK_VALUE(counts.scalar_type() == at::kInt && counts.device() == logits.device() && counts.dim() == 1 && counts.size(0) == experts &&

@@ -9,7 +9,7 @@ columns by the layer's own quantiser, FP32 accumulation, one rounding to the act
 Every call enqueues on torch's current stream of the operands' device and may be captured in a CUDA graph; nothing is kept
 between calls.  There is no CPU implementation.  Sizes are up to 2^26; weights (and codes) need rows that are contiguous and
 start on 16-byte boundaries, so a width that is no multiple of 16 is stored with padded rows; activations may have any strides.
-Bad operands raise ValueError, failures of the C ABI RuntimeError.
+Bad operands raise ValueError, operands that carry a forward-mode tangent NotImplementedError, failures of the C ABI RuntimeError.
 """
 from __future__ import annotations
 

@@ -502,3 +502,29 @@ def test_second_derivatives_are_refused_in_every_call():
                 again()
         (dx,) = torch.autograd.grad(linear(x, w, ws), x, dy.detach(), create_graph=True)       # depends on nothing that is differentiated
         assert torch.equal(dx, torch.autograd.grad(linear(x, w, ws), x, dy.detach())[0])
+
+
+def test_forward_mode_is_refused():
+    """No output without its tangent: neither for operands that require a gradient nor for those that do not, nor in a backward pass."""
+    from torch.autograd import forward_ad
+    from netra_kernel_b200 import torch_ops  # noqa: F401
+    w, ws = make_weight(64, 256, 1)
+    x, z = torch.randn(4, 256, device="cuda"), torch.randn(5, 16, device="cuda")
+    counts, one = torch.ones(16, dtype=torch.int32, device="cuda"), torch.ones((), device="cuda")
+    codes, scale = dense.quantize_rows(x)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))      # noqa: E731
+        leaf, dz = x.clone().requires_grad_(), z.clone().requires_grad_()
+        for call in (lambda: dense.fp8_linear(dual(x), w, ws), lambda: dense.fp8_linear(dual(leaf), w, ws), lambda: dense.fp8_linear(x, w, dual(ws)),
+                     lambda: dense.fp8_linear(dual(x).t().contiguous().t(), w, ws), lambda: dense.fp8_linear(dual(x)[:0], w, ws),
+                     lambda: dense.quantize_rows(dual(x)), lambda: dense.block_scaled_matmul(codes, dual(scale), w, ws),
+                     lambda: dense.block_scaled_matmul(codes, scale, w, ws, out=dual(torch.zeros(4, 64, device="cuda"))),
+                     lambda: torch.autograd.grad(dense.fp8_linear(leaf, w, ws), leaf, dual(torch.ones(4, 64, device="cuda"))),
+                     lambda: balance.balance_loss(dual(z), counts), lambda: balance.balance_loss(dual(dz), counts),
+                     lambda: balance.balance_loss_grad(one, dual(z), counts), lambda: balance.balance_loss_grad(dual(one), z, counts),
+                     lambda: torch.autograd.grad(balance.balance_loss(dz, counts), dz, dual(one)),
+                     lambda: torch.ops.netra.fp8_linear(dual(x), w, ws), lambda: torch.ops.netra.balance_loss(dual(z), counts)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        plain = dense.fp8_linear(x, w, ws)                                # nothing else changes inside a dual level
+    assert torch.equal(plain, dense.fp8_linear(x, w, ws))
