@@ -121,6 +121,8 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
                                            ws.const_data_ptr<float>(), pitch_of(ws), transpose_weight, (uint32_t)m, (uint32_t)w.size(0),
                                            (uint32_t)w.size(1), stream_of(a)),
              "dense_fp8_matmul_launch");
+    // written in place: autograd may have saved it for some backward pass (an inference tensor it cannot)
+    if (out_given.has_value() && !out.is_inference()) torch::autograd::impl::bump_version(out);
   }
   return out;
 }

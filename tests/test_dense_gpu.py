@@ -528,3 +528,22 @@ def test_forward_mode_is_refused():
                 call()
         plain = dense.fp8_linear(x, w, ws)                                # nothing else changes inside a dual level
     assert torch.equal(plain, dense.fp8_linear(x, w, ws))
+
+
+def test_a_given_output_counts_as_written():
+    """A tensor that autograd keeps for a backward pass is not the same one after it has been an output."""
+    w, ws = make_weight(64, 256, 1)
+    codes, scale = dense.quantize_rows(torch.randn(4, 256, device="cuda"))
+    frame, leaf = torch.ones(6, 64, device="cuda"), torch.ones(4, 64, device="cuda").requires_grad_()
+    product = (leaf * frame[1:5]).sum()
+    assert dense.block_scaled_matmul(codes, scale, w, ws, out=frame[1:5]).data_ptr() == frame[1:5].data_ptr()
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        product.backward()
+    before = frame._version
+    dense.block_scaled_matmul(codes[:0], scale[:0], w, ws, out=frame[:0])
+    assert frame._version == before                                   # nothing was written
+    with torch.inference_mode():
+        kept = torch.zeros(4, 64, device="cuda")
+        dense.block_scaled_matmul(codes, scale, w, ws, out=kept)
+    dense.block_scaled_matmul(codes, scale, w, ws, out=kept)
+    assert torch.equal(kept, frame[1:5])
