@@ -469,8 +469,9 @@ int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, 
                                   uint32_t transpose_w, uint32_t m, uint32_t w_rows, uint32_t w_cols, void* workspace,
                                   uint64_t workspace_bytes, cudaStream_t stream);
 
-/* The current device's status words of the dense kernels (synchronises): word 0 is 0, or the role whose bounded wait ran out in some
- * call since the words were last read (reading clears them); the output of that call is not valid. */
+/* The current device's status words of the dense kernels: word 0 is 0, or the role whose bounded wait ran out in some call since
+ * the words were last read (reading clears them); the output of that call is not valid.  Waits for everything enqueued on the
+ * device, on every stream, so it is not allowed while a stream is being captured. */
 int netra_dense_status(uint32_t status_out[4]);
 
 /* ------------------------------------------------------------------ router load and balance loss

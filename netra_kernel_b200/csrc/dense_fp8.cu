@@ -13,8 +13,12 @@ namespace netra {
 
 enum : uint32_t { kDenseBf16 = 0, kDenseF16 = 1, kDenseF32 = 2 };
 
-// Where a bounded wait of a dense kernel ran out (kStatus* codes); read by netra_dense_status.
+// Where a bounded wait of a dense kernel ran out (kStatus* codes); read by netra_dense_status, which moves the words into
+// g_dense_taken in one step each, so that a code written meanwhile is there for the next reading.
 __device__ uint32_t g_dense_status[4];
+__device__ uint32_t g_dense_taken[4];
+
+extern "C" __global__ void netra_dense_take_status_sm100() { g_dense_taken[threadIdx.x] = atomicExch(&g_dense_status[threadIdx.x], 0u); }
 
 __device__ __forceinline__ float dense_load(const void* p, uint32_t dtype, size_t i) {
   if (dtype == kDenseBf16) return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
@@ -545,7 +549,7 @@ int encode_output(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, ui
   return 0;
 }
 
-std::mutex g_dense_mutex;
+std::mutex g_dense_mutex, g_dense_taken_mutex;
 bool g_dense_pair_ok[kMaxDevices] = {};   // the pair kernels were built with the register allocation they assume
 int g_dense_sms[kMaxDevices] = {};      // SM count once the kernels of a device are set up
 
@@ -788,9 +792,12 @@ int netra_dense_fp8_linear_launch(void* out, uint64_t out_pitch, const void* x, 
 
 int netra_dense_status(uint32_t status_out[4]) {
   if (status_out == nullptr) return fail("dense_status: null pointer");
-  cudaError_t e = cudaMemcpyFromSymbol(status_out, g_dense_status, 16);
-  const uint32_t clear[4] = {0, 0, 0, 0};
-  if (e == cudaSuccess && (status_out[0] | status_out[1] | status_out[2] | status_out[3])) e = cudaMemcpyToSymbol(g_dense_status, clear, 16);
+  cudaError_t e = cudaDeviceSynchronize();       // the copy below is ordered behind the default stream only
+  if (e != cudaSuccess) return fail_cuda("dense status", e);
+  std::lock_guard<std::mutex> lock(g_dense_taken_mutex);
+  netra_dense_take_status_sm100<<<1, 4>>>();
+  if (int rc = check_launch("dense status launch")) return rc;
+  e = cudaMemcpyFromSymbol(status_out, g_dense_taken, 16);
   return e == cudaSuccess ? 0 : fail_cuda("dense status", e);
 }
 

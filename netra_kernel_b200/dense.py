@@ -54,9 +54,12 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
 
 def check_status(device: Optional[torch.device] = None) -> None:
-    """Raises if a bounded wait inside a dense kernel of the device ran out (synchronises)."""
+    """Raises if a bounded wait inside a dense kernel of the device ran out.  Waits for all work enqueued on the device, on every
+    stream; refused while a graph is being captured."""
     words = (ctypes.c_uint32 * 4)()
     with torch.cuda.device(device) if device is not None else nullcontext():
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("check_status waits for the device, which a stream that is being captured does not allow")
         abi.check(abi.load().netra_dense_status(ctypes.byref(words)), "dense_status")
     if any(words):
         raise abi.NetraError(f"device status words {list(words)}: a bounded wait expired inside a dense FP8 product")

@@ -547,3 +547,24 @@ def test_a_given_output_counts_as_written():
         dense.block_scaled_matmul(codes, scale, w, ws, out=kept)
     dense.block_scaled_matmul(codes, scale, w, ws, out=kept)
     assert torch.equal(kept, frame[1:5])
+
+
+def test_status_waits_for_every_stream():
+    """A product still running on a stream of its own has not reported yet."""
+    w, ws = make_weight(64, 256, 1)
+    x, side = torch.randn(300, 256, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)                                # about 0.2 s
+        dense.fp8_linear(x, w, ws)
+        done = side.record_event()
+    dense.check_status()
+    assert done.query()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dense.fp8_linear(x, w, ws)
+        with pytest.raises(RuntimeError, match="captured"):
+            dense.check_status()
+    graph.replay()
+    dense.check_status()
+    assert torch.equal(y, dense.fp8_linear(x, w, ws))
