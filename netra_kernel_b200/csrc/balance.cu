@@ -316,6 +316,7 @@ int balance_check(const char* what, const void* z, uint32_t dtype, uint64_t pitc
   if (tokens == 0 || tokens > (1ull << 40)) return bad("tokens out of range");
   if (tokens > 1 && pitch < experts) return bad("a row pitch is smaller than the row");
   if ((uintptr_t)z % dense_element_bytes(dtype)) return bad("logits are not aligned to their element");
+  if ((uintptr_t)counts % 4) return bad("counts are not aligned to their element");
   return 0;
 }
 
@@ -359,6 +360,7 @@ int netra_expert_counts_launch(int32_t* counts_i32, const void* ids, uint32_t id
   if (tokens > (1ull << 40) || slots > 1024 || tokens * slots > 0x7fffffffull) return fail("expert_counts: at most 2^31 - 1 choices of 1024 slots");
   if (tokens > 1 && id_pitch < slots) return fail("expert_counts: the row pitch is smaller than the row");
   if ((uintptr_t)ids % id_bytes) return fail("expert_counts: ids are not aligned to their element");
+  if ((uintptr_t)counts_i32 % 4) return fail("expert_counts: counts are not aligned to their element");
   const uint64_t pairs = tokens * slots;
   if (pairs <= kCountsClusterPairs)
     return launched("expert_counts launch",
@@ -381,6 +383,7 @@ int netra_balance_loss_launch(float* loss_f32, float* scale_f32, const void* log
                               cudaStream_t stream) {
   if (int rc = balance_check("balance_loss", logits, dtype, pitch, counts_i32, tokens, experts)) return rc;
   if (!loss_f32 || !scale_f32) return fail("balance_loss: null pointer");
+  if ((uintptr_t)loss_f32 % 4 || (uintptr_t)scale_f32 % 4) return fail("balance_loss: an address is not aligned to its element");
   const uint64_t needed = netra_balance_loss_workspace_bytes(tokens, experts);
   if (needed > 0 && (!workspace || workspace_bytes < needed || (uintptr_t)workspace % 16)) return fail("balance_loss: workspace missing, too small or not 16-byte aligned");
   const bool aligned = balance_aligned(logits, pitch, dtype, experts);
@@ -414,6 +417,7 @@ int netra_balance_loss_grad_launch(void* grad, uint64_t grad_pitch, const void* 
   if (!grad || !scale_f32 || !upstream_f32) return fail("balance_loss_grad: null pointer");
   if (tokens > 1 && grad_pitch < experts) return fail("balance_loss_grad: a row pitch is smaller than the row");
   if ((uintptr_t)grad % dense_element_bytes(dtype)) return fail("balance_loss_grad: the gradient is not aligned to its element");
+  if ((uintptr_t)scale_f32 % 4 || (uintptr_t)upstream_f32 % 4) return fail("balance_loss_grad: an address is not aligned to its element");
   const uint32_t grid = balance_blocks(tokens);
   const bool aligned = balance_aligned(logits, pitch, dtype, experts) && balance_aligned(grad, grad_pitch, dtype, experts);
   cudaError_t launch = cudaSuccess;

@@ -650,6 +650,7 @@ int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, floa
                                      uint32_t k, cudaStream_t stream) {
   if (!codes_fp8 || !scale_f32) return fail("dense_quantize_rows: null pointer");
   if (int rc = check_quantize_operands(x, x_dtype, x_pitch, m, k)) return rc;
+  if ((uintptr_t)scale_f32 % 4) return fail("dense_quantize_rows: the scales are not aligned to their element");
   if (m > 1 && codes_pitch < k) return fail("dense_quantize_rows: a row pitch is smaller than the row");
   const uint64_t blocks = (k + 127) / 128;
   // four rows per lane once that still leaves every SM a few thousand lanes; below, one row each for the shortest chain

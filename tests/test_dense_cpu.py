@@ -99,3 +99,21 @@ def test_operators_by_name_trace_without_a_device():
         loss = torch.ops.netra.balance_loss(z, counts)
         dz = torch.ops.netra.balance_loss_grad(loss, z, counts)
         assert loss.shape == () and loss.dtype == torch.float32 and dz.shape == z.shape
+
+
+def test_c_entries_refuse_addresses_off_their_element():
+    """Every address that a kernel reads or writes by whole elements; refused on the host, nothing is launched."""
+    lib = abi.load()
+    p = 4096                                 # never dereferenced
+    size = lib.netra_balance_loss_workspace_bytes(5000, 16)
+    quant = lambda s=p: lib.netra_dense_quantize_rows_launch(p, 128, s, 1, 2, p, 0, 128, 2, 128, None)                                   # noqa: E731
+    matmul = lambda s=p, ws=p, out=p: lib.netra_dense_fp8_matmul_launch(out, 2, 64, p, 128, s, 1, 2, p, 128, ws, 1, 0, 2, 64, 128, None)   # noqa: E731
+    cnt = lambda c=p, ids=p, b=8: lib.netra_expert_counts_launch(c, ids, b, 8, None, 2, 8, 256, None)                                    # noqa: E731
+    loss = lambda l=p, sc=p, z=p, c=p, t=5000: lib.netra_balance_loss_launch(l, sc, z, 2, 16, c, None, p, size, t, 16, None)             # noqa: E731
+    grad = lambda g=p, z=p, c=p, s=p, u=p: lib.netra_balance_loss_grad_launch(g, 16, z, 2, 16, c, None, s, u, 2, 16, None)               # noqa: E731
+    for call, names in [(quant, ["s"]), (matmul, ["s", "ws", "out"]), (cnt, ["c", "ids"]), (loss, ["l", "sc", "z", "c"]), (grad, ["g", "z", "c", "s", "u"])]:
+        for name in names:
+            for off in (1, 2, 3):
+                assert call(**{name: p + off}) == -1 and "aligned" in lib.netra_moe_last_error().decode(), (call, name, off)
+    for off in (2, 6):
+        assert loss(t=2, c=p + off) == -1 and "aligned" in lib.netra_moe_last_error().decode()      # the form without a workspace
