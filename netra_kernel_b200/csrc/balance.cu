@@ -145,11 +145,24 @@ struct BalLane {
   }
 };
 
-// e^x for x <= 0: a hardware base-2 exponential of the rounded product (errors of 2 steps, and |x| 2^-24 from the rounding)
-__device__ __forceinline__ float exp_nonpositive(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
-  return r;
+// e^x = 2^h (1 + r) for x <= 0, with h = fl(x log2 e) and r = x - h ln 2, which is below 2^-17 and so leaves r^2 / 2 out; ln 2 in
+// two parts, as in Cody and Waite's reductions.  The rounding of h alone would cost |x| 2^-24 (a probability of e^-80 off by 60
+// units of 2^-24); 2^h is the hardware's, within two steps.  Two elements share their multiply-adds.  Loss and gradient of
+// 16384 x 256 BF16: 18.8 us, 20.5 us with expf() instead; of 16384 x 512 FP32: 22.7 us, 24.7 us, 23.5 us one element at a time.
+__device__ __forceinline__ float2 exp_nonpositive2(float a, float b) {
+  auto finite = [](float x) {               // keeps a NaN; e^-200 is 0
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-200.0f));
+    return r;
+  };
+  auto both = [](float c) { return make_float2(c, c); };
+  const float2 x = make_float2(finite(a), finite(b));
+  const float2 h = fma2(x, both(1.4426950408889634f), both(-0.0f));
+  const float2 r = fma2(h, both(1.9046543e-9f), fma2(h, both(-0.69314718f), x));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(h.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(h.y));
+  return fma2(e, r, e);
 }
 
 // v: a row's logits -> its exponentials; returns sum_e c_e p_e in every lane, inv = 1 / sum of the exponentials
@@ -162,10 +175,13 @@ __device__ __forceinline__ float bal_row(float v[kPer], const float c[kPer], flo
   const float shift = mx == -INFINITY ? 0.0f : mx;
   float sum = 0.0f, dot = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    v[i] = exp_nonpositive(v[i] - shift);
-    sum += v[i];
-    dot = fmaf(v[i], c[i], dot);
+  for (int i = 0; i < kPer; i += 2) {
+    const float2 e = exp_nonpositive2(v[i] - shift, v[i + 1] - shift);
+    v[i] = e.x; v[i + 1] = e.y;
+    sum += e.x;
+    sum += e.y;
+    dot = fmaf(e.x, c[i], dot);
+    dot = fmaf(e.y, c[i + 1], dot);
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {

@@ -262,3 +262,27 @@ def test_refusals():
     ]:
         with pytest.raises(ValueError, match=why):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_improbable_experts_keep_their_precision(dtype):
+    """Logits whose differences are exact, one likely expert without a choice, the others up to e^-80 as likely.  In units of 2^-24 a
+    gradient is off by at most: 5 for its exponential (two steps of FP32 and a rounding) and 5 for the row's (all but the likely one,
+    whose exponential is 1), 9 additions in the row's sum and as many in that of the counts, 2 quotients, 3 for f - d and the loss's
+    factor, 5 products; 38 together, and half a step of its type.  The rounding of the exponent alone (gap * log2 e, half a step of
+    up to 2^-17) would cost up to 90."""
+    t, e = 300, 64
+    gap = torch.randint(8, 640, (t, e), generator=torch.Generator().manual_seed(9)).double() / 8
+    if dtype == torch.bfloat16:
+        gap = gap.floor()                                            # whole numbers below 128 are BF16 values
+    gap[:, 0] = 0
+    counts = torch.full((e,), 1000, dtype=torch.int32)
+    counts[0] = 0
+    z = (-gap).to(dtype).cuda().requires_grad_()
+    assert torch.equal(z.detach().cpu().double(), -gap)
+    (grad,) = torch.autograd.grad(balance.balance_loss(z, counts.cuda()), z)
+    p, f = torch.softmax(-gap, dim=1), counts.double() / counts.sum()
+    want = e / t * p * (f - (p @ f)[:, None])
+    tol = (38 * 2.0 ** -24 + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0)) * want.abs()
+    err = (grad.cpu().double() - want).abs()[:, 1:]
+    assert bool((err <= tol[:, 1:]).all()), float((err / want.abs()[:, 1:]).max() * 2 ** 24)
