@@ -94,6 +94,8 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
                            at::ScalarType out_dtype, const std::optional<Tensor>& out_given) {
   TORCH_CHECK_VALUE(a.is_cuda() && a.scalar_type() == at::kFloat8_e4m3fn && a.dim() == 2, "a must be a float8_e4m3fn CUDA matrix");
   check_weight(w, ws, a.device());
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(a.requires_grad() || a_scale.requires_grad()),
+                    "a product of ready codes carries no gradient, so a and a_scale must not require one (fp8_linear differentiates)");
   refuse_tangent(a);
   refuse_tangent(a_scale);
   const int64_t m = a.size(0), k = w.size(transpose_weight ? 0 : 1), n = w.size(transpose_weight ? 1 : 0);

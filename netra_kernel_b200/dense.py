@@ -30,7 +30,7 @@ def quantize_rows(x: torch.Tensor):
     """``x`` [..., K] (BF16, FP16 or FP32) -> (E4M3 codes [M, K], FP32 scales [M, ceil(K/128)]), M the product of the leading
     sizes: ``scale = max(amax of the row's 128 columns, 1e-10) * fl(1/448)``, ``code = e4m3_rne_sat(x * fl(1/scale))``.
     The rows of the codes are padded to 128 bytes and the scales stored block by block, the forms the product reads best.
-    A NaN stays at its element; an infinity makes its block's scale infinite."""
+    A NaN stays at its element; an infinity makes its block's scale infinite.  Codes and scales carry no gradient."""
     return _ext.quantize_rows(x)
 
 
@@ -39,7 +39,8 @@ def block_scaled_matmul(a: torch.Tensor, a_scale: torch.Tensor, weight: torch.Te
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a`` [M, K] E4M3 with scales [M, ceil(K/128)] times a block-scaled weight: ``a @ weight.T`` [M, N] for ``weight``
     [N, K], or with ``transpose_weight`` ``a`` [M, N] times ``weight`` as it is stored -> [M, K].  ``weight_scale`` is
-    [ceil(N/128), ceil(K/128)] either way.  ``out`` (row-major) takes the result in its own type."""
+    [ceil(N/128), ceil(K/128)] either way.  ``out`` (row-major) takes the result in its own type.  The product carries
+    no gradient and refuses operands that require one, unless gradients are off."""
     return _ext.block_scaled_matmul(a, a_scale, weight, weight_scale, transpose_weight, out_dtype, out)
 
 

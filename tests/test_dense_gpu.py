@@ -568,3 +568,16 @@ def test_status_waits_for_every_stream():
     graph.replay()
     dense.check_status()
     assert torch.equal(y, dense.fp8_linear(x, w, ws))
+
+
+def test_a_product_of_ready_codes_refuses_operands_that_require_a_gradient():
+    w, ws = make_weight(64, 256, 1)
+    codes, scale = dense.quantize_rows(torch.randn(4, 256, device="cuda").requires_grad_())
+    assert not codes.requires_grad and not scale.requires_grad
+    learned, learned_codes = scale.clone().requires_grad_(), codes.clone().requires_grad_()
+    for a, s in ((codes, learned), (learned_codes, scale), (codes, learned * 2)):
+        with pytest.raises(ValueError, match="gradient"):
+            dense.block_scaled_matmul(a, s, w, ws)
+        with torch.no_grad():
+            y = dense.block_scaled_matmul(a, s, w, ws)
+        assert not y.requires_grad and torch.equal(y, dense.block_scaled_matmul(a.detach(), s.detach(), w, ws))
