@@ -9,11 +9,15 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/netra_moe.h"
 
@@ -161,15 +165,44 @@ Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool trans
 
 // A leaf keeps its gradient node, with the stream it was made on, for as long as any graph of it lives.  If that was the default
 // stream, a backward pass captured on another one makes torch tie the two together, which CUDA forbids and which invalidates the
-// capture; so such a call is refused while the capture can still be ended.
+// capture; so such a call is refused while the capture can still be ended: the forward call of the leaf itself, and, since the leaf
+// may lie behind other operations, the operator's step of the backward pass.
+bool capturing() { return c10::cuda::device_count() > 0 && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+
+void refuse_default_stream(torch::autograd::Node& leaf) {
+  const auto made_on = leaf.stream();
+  TORCH_CHECK(!made_on.has_value() || made_on->id() != 0 || *made_on == c10::cuda::getCurrentCUDAStream(made_on->device_index()).unwrap(),
+              "an eager graph of this leaf, made on the default stream, is still alive: drop it (its loss and outputs) before capturing a "
+              "forward and backward pass of the same leaf, or capture with a fresh leaf (or, for the forward pass alone, under torch.no_grad())");
+}
+
 void check_capture(const Tensor& x) {
   if (x.grad_fn()) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
-  if (!node || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  const auto made_on = node->stream();
-  TORCH_CHECK(!made_on.has_value() || made_on->id() != 0 || *made_on == c10::cuda::getCurrentCUDAStream(x.device().index()).unwrap(),
-              "an eager graph of this leaf, made on the default stream, is still alive: drop it (its loss and outputs) before capturing a "
-              "forward and backward pass of the same leaf, or capture with a fresh leaf");
+  if (node && capturing()) refuse_default_stream(*node);
+}
+
+// Called in a backward step: looks at every leaf that this backward pass will reach from here.
+void check_captured_backward() {
+  const auto node = torch::autograd::get_current_node();
+  if (!node || !capturing()) return;
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();       // empty: every node
+  std::unordered_set<torch::autograd::Node*> seen;
+  std::vector<torch::autograd::Node*> stack{node.get()};
+  while (!stack.empty()) {
+    const auto* at = stack.back();
+    stack.pop_back();
+    for (const auto& edge : at->next_edges()) {
+      auto* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (wanted && !wanted->empty()) {
+        const auto it = wanted->find(next);
+        if (it == wanted->end() || !it->second.should_execute()) continue;
+      }
+      if (dynamic_cast<torch::autograd::AccumulateGrad*>(next)) refuse_default_stream(*next);
+      stack.push_back(next);
+    }
+  }
 }
 
 struct LinearGradFunction : torch::autograd::Function<LinearGradFunction> {
@@ -183,6 +216,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     return linear(x, w, ws, false);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    check_captured_backward();
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
     return {at::GradMode::is_enabled() ? LinearGradFunction::apply(dy, saved[0], saved[1]) : linear(dy, saved[0], saved[1], true), Tensor(), Tensor()};
@@ -274,6 +308,7 @@ struct BalanceFunction : torch::autograd::Function<BalanceFunction> {
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    check_captured_backward();
     const auto saved = ctx->get_saved_variables();
     const Tensor &z = saved[0], &counts = saved[1], &scale = saved[2];
     const auto mask = saved[3].defined() ? std::optional<Tensor>(saved[3]) : std::nullopt;
@@ -317,6 +352,7 @@ Tensor balance_loss(const Tensor& logits, const Tensor& counts, const std::optio
 PYBIND11_MODULE(_netra_torch, m) {
   // argument errors are ValueError, errors of the C ABI RuntimeError; the interpreter lock is released during a call
   m.def("check_weight", torch::wrap_pybind_function_no_gil(check_weight_on));
+  m.def("check_captured_backward", torch::wrap_pybind_function_no_gil(check_captured_backward));
   m.def("quantize_rows", torch::wrap_pybind_function_no_gil(quantize_rows));
   m.def("block_scaled_matmul", torch::wrap_pybind_function_no_gil(block_scaled_matmul));
   m.def("fp8_linear", torch::wrap_pybind_function_no_gil(fp8_linear));

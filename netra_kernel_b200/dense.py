@@ -7,9 +7,11 @@ columns by the layer's own quantiser, FP32 accumulation, one rounding to the act
     y = fp8_linear(x, weight, weight_scale)                           # both; differentiable with respect to x
 
 Every call enqueues on torch's current stream of the operands' device and may be captured in a CUDA graph; nothing is kept
-between calls.  There is no CPU implementation.  Sizes are up to 2^26; weights (and codes) need rows that are contiguous and
-start on 16-byte boundaries, so a width that is no multiple of 16 is stored with padded rows; activations may have any strides.
-Bad operands raise ValueError, operands that carry a forward-mode tangent NotImplementedError, failures of the C ABI RuntimeError.
+between calls.  A backward pass cannot be captured while an eager graph of one of its leaves, made on the default stream, is alive
+(RuntimeError; an operand that is such a leaf is refused in the forward call, unless under ``torch.no_grad()``).  There is no CPU
+implementation.  Sizes are up to 2^26; weights (and codes) need rows that are contiguous and start on 16-byte boundaries, so a
+width that is no multiple of 16 is stored with padded rows; activations may have any strides.  Bad operands raise ValueError,
+operands that carry a forward-mode tangent NotImplementedError, failures of the C ABI RuntimeError.
 """
 from __future__ import annotations
 

@@ -156,6 +156,8 @@ def _keep_weight(ctx, inputs, output) -> None:
 
 
 def _linear_backward(ctx, grad):
+    from . import abi
+    abi.torch_binding().check_captured_backward()
     return torch.ops.netra.fp8_linear_input_grad(grad, *ctx.saved_tensors), None, None
 
 
@@ -202,6 +204,8 @@ def _keep_routing(ctx, inputs, output) -> None:
 
 
 def _balance_backward(ctx, upstream):
+    from . import abi
+    abi.torch_binding().check_captured_backward()
     logits, counts, *mask = ctx.saved_tensors
     return torch.ops.netra.balance_loss_grad(upstream, logits, counts, mask[0] if ctx.has_mask else None), None, None
 

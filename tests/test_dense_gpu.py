@@ -581,3 +581,50 @@ def test_a_product_of_ready_codes_refuses_operands_that_require_a_gradient():
         with torch.no_grad():
             y = dense.block_scaled_matmul(a, s, w, ws)
         assert not y.requires_grad and torch.equal(y, dense.block_scaled_matmul(a.detach(), s.detach(), w, ws))
+
+
+def test_captured_backward_beside_a_living_eager_graph_of_a_leaf_behind_the_operand_is_refused():
+    """The leaf may lie behind other operations, and the operators by name know it only in their backward step; what does not reach
+    that leaf is captured as usual."""
+    from netra_kernel_b200 import torch_ops  # noqa: F401
+    w, ws = make_weight(64, 128, 1)
+    x, router = torch.randn(4, 128, device="cuda"), torch.randn(64, 64, device="cuda").requires_grad_()
+    counts = torch.arange(64, dtype=torch.int32, device="cuda")
+    hidden = dense.fp8_linear(x, w, ws)
+    warm = torch.zeros(4, 64, device="cuda").requires_grad_()          # torch sets up its matrix products, which a capture does not allow
+    torch.autograd.grad((warm @ torch.ones_like(router)).sum(), warm)
+    alive = hidden @ router                                            # an eager graph of the router
+    leaf = x.clone().requires_grad_()
+    alive_linear = leaf * 2
+    fresh = torch.zeros(4, 64, device="cuda").requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for loss_of in (balance.balance_loss, torch.ops.netra.balance_loss):
+            loss = loss_of(hidden @ router, counts)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                torch.autograd.grad(loss, router)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                loss_of(hidden @ router, counts).backward()
+        for linear in (dense.fp8_linear, torch.ops.netra.fp8_linear):
+            y = linear(leaf + 1, w, ws)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                torch.autograd.grad(y.sum(), leaf)
+        y = torch.ops.netra.fp8_linear(leaf, w, ws)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            torch.autograd.grad(y.sum(), leaf)
+        loss = balance.balance_loss((hidden + fresh) @ router, counts)
+        (d_fresh,) = torch.autograd.grad(loss, fresh)
+    graph.replay()
+    torch.cuda.synchronize()
+    again = torch.zeros(4, 64, device="cuda").requires_grad_()
+    (want,) = torch.autograd.grad(balance.balance_loss((hidden + again) @ router, counts), again)
+    assert torch.equal(d_fresh, want)
+    del alive, alive_linear, y, loss
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(torch.ops.netra.balance_loss(hidden @ router, counts), router)
+        (got_x,) = torch.autograd.grad(torch.ops.netra.fp8_linear(leaf, w, ws).sum(), leaf)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, torch.autograd.grad(balance.balance_loss(hidden @ router, counts), router)[0])
+    assert torch.equal(got_x, torch.autograd.grad(dense.fp8_linear(leaf, w, ws).sum(), leaf)[0])
