@@ -4,6 +4,7 @@
 // the host's share decides what a call costs: the same path through ctypes took 26 us per fp8_linear call and 130 us with its
 // gradient (Python autograd function).  Everything below the C ABI of include/netra_moe.h is unchanged; C callers need none of this.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -116,6 +117,10 @@ Tensor block_scaled_matmul(const Tensor& a, const Tensor& a_scale, const Tensor&
     TORCH_CHECK_VALUE(out.device() == a.device() && is_activation(out.scalar_type()) && out.dim() == 2 && out.size(0) == m && out.size(1) == n &&
                           (out.stride(1) == 1 || n == 1) && (out.stride(0) >= n || m <= 1) && !out.requires_grad(),
                       "out must be a row-major [M, N] matrix of BF16, FP16 or FP32 on a's device");
+    for (const Tensor* operand : {&a, &a_scale, &w, &ws}) {        // as far as torch can tell without walking strided views
+      const auto overlap = at::get_overlap_status(out, *operand);
+      TORCH_CHECK_VALUE(overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial, "out must not share memory with an operand");
+    }
   } else {
     TORCH_CHECK_VALUE(is_activation(out_dtype), "out_dtype must be bfloat16, float16 or float32");
     out = at::empty({m, n}, a.options().dtype(out_dtype));

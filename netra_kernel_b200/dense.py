@@ -41,7 +41,7 @@ def block_scaled_matmul(a: torch.Tensor, a_scale: torch.Tensor, weight: torch.Te
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a`` [M, K] E4M3 with scales [M, ceil(K/128)] times a block-scaled weight: ``a @ weight.T`` [M, N] for ``weight``
     [N, K], or with ``transpose_weight`` ``a`` [M, N] times ``weight`` as it is stored -> [M, K].  ``weight_scale`` is
-    [ceil(N/128), ceil(K/128)] either way.  ``out`` (row-major) takes the result in its own type.  The product carries
+    [ceil(N/128), ceil(K/128)] either way.  ``out`` (row-major, no memory of an operand) takes the result in its own type.  The product carries
     no gradient and refuses operands that require one, unless gradients are off."""
     return _ext.block_scaled_matmul(a, a_scale, weight, weight_scale, transpose_weight, out_dtype, out)
 

@@ -628,3 +628,22 @@ def test_captured_backward_beside_a_living_eager_graph_of_a_leaf_behind_the_oper
     torch.cuda.synchronize()
     assert torch.equal(got, torch.autograd.grad(balance.balance_loss(hidden @ router, counts), router)[0])
     assert torch.equal(got_x, torch.autograd.grad(dense.fp8_linear(leaf, w, ws).sum(), leaf)[0])
+
+
+def test_an_output_in_an_operands_memory_is_refused():
+    """Other blocks still read what the first ones would overwrite.  Neighbours in one buffer are fine."""
+    w, ws = make_weight(64, 256, 1)
+    codes, scale = dense.quantize_rows(torch.randn(4, 256, device="cuda"))
+    wide, wide_scale = make_weight(256, 128, 2)
+    tall = dense.quantize_rows(torch.randn(64, 128, device="cuda"))
+    square_scale = torch.ones(4, 2, device="cuda")
+    few, few_scale = make_weight(2, 256, 3)
+    for call in (lambda: dense.block_scaled_matmul(codes, scale, w, ws, out=codes.view(torch.float32)),
+                 lambda: dense.block_scaled_matmul(codes, square_scale, few, few_scale, out=square_scale),
+                 lambda: dense.block_scaled_matmul(*tall, wide, wide_scale, out=wide.view(torch.bfloat16).view(64, 256))):
+        with pytest.raises(ValueError, match="memory"):
+            call()
+    buffer = torch.zeros(2048, dtype=torch.uint8, device="cuda")
+    near, out = buffer[:1024].view(torch.float8_e4m3fn).view(4, 256), buffer[1024:].view(torch.float32).view(4, 64)
+    near.view(torch.uint8).copy_(codes.view(torch.uint8))
+    assert torch.equal(dense.block_scaled_matmul(near, scale, w, ws, out=out), dense.block_scaled_matmul(codes, scale, w, ws, out_dtype=torch.float32))
