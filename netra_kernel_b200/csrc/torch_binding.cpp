@@ -143,7 +143,9 @@ Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool trans
   const Tensor x = as_rows(input, "x");
   const int64_t m = x.size(0), k = w.size(transposed ? 0 : 1), n = w.size(transposed ? 1 : 0);
   check_sizes(m, w);
-  Tensor out = at::empty({m, n}, x.options());
+  auto shape = input.sizes().vec();
+  shape.back() = n;
+  Tensor out = at::empty(shape, x.options());          // not a view of a matrix, which autograd would not let a caller modify in place
   if (m > 0) {
     const c10::cuda::CUDAGuard guard(x.device());
     uint64_t bytes = 0;
@@ -157,10 +159,7 @@ Tensor linear(const Tensor& input, const Tensor& w, const Tensor& ws, bool trans
                                            (uint32_t)w.size(1), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(x)),
              "dense_fp8_linear_launch");
   }
-  if (input.dim() == 2) return out;
-  auto shape = input.sizes().vec();
-  shape.back() = n;
-  return out.view(shape);
+  return out;
 }
 
 // The gradients have no derivatives of their own.  A backward pass that is itself being differentiated (create_graph) computes its

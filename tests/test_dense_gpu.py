@@ -647,3 +647,30 @@ def test_an_output_in_an_operands_memory_is_refused():
     near, out = buffer[:1024].view(torch.float8_e4m3fn).view(4, 256), buffer[1024:].view(torch.float32).view(4, 64)
     near.view(torch.uint8).copy_(codes.view(torch.uint8))
     assert torch.equal(dense.block_scaled_matmul(near, scale, w, ws, out=out), dense.block_scaled_matmul(codes, scale, w, ws, out_dtype=torch.float32))
+
+
+def test_results_may_be_modified_in_place():
+    """As any linear layer's: a bias or an activation on the spot, whatever the leading sizes, with gradients."""
+    from netra_kernel_b200 import torch_ops  # noqa: F401
+    w, ws = make_weight(48, 128, 1)
+    bias, dy = torch.randn(48, device="cuda"), torch.randn(12, 48, device="cuda")
+    flat = torch.randn(12, 128, device="cuda")
+    for linear in (dense.fp8_linear, torch.ops.netra.fp8_linear):
+        plain = flat.clone().requires_grad_()
+        want = torch.relu(linear(plain, w, ws) + bias)
+        (want_dx,) = torch.autograd.grad(want, plain, dy)
+        for shape in ((12,), (2, 6), (3, 1, 4)):
+            x = flat.view(*shape, 128).clone().requires_grad_()
+            y = linear(x, w, ws)
+            y += bias
+            y.relu_()
+            assert y.shape == (*shape, 48) and torch.equal(y.view(12, 48), want)
+            (dx,) = torch.autograd.grad(y, x, dy.view(*shape, 48))
+            assert torch.equal(dx.view(12, 128), want_dx)
+    x = flat[0].clone().requires_grad_()
+    y = dense.fp8_linear(x, w, ws)
+    y += bias
+    y.sum().backward()
+    loss = balance.balance_loss(flat.clone().requires_grad_(), torch.ones(128, dtype=torch.int32, device="cuda"))
+    loss *= 0.5
+    loss.backward()
