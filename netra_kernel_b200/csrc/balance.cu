@@ -318,9 +318,10 @@ netra_balance_loss_grad_sm100(T* grad, uint64_t grad_pitch, const T* z, uint64_t
 namespace {
 
 // Up to here one cluster of eight blocks does it, without clearing anything first (one cluster against many blocks behind a
-// memset: counts of 2,048 choices 2.7 us against 5.0 us, of 65,536 choices 4.8 us against 6.2 us; loss of 256 tokens and 256
-// experts 3.3 us against 6.4 us, of 2,048 tokens 8.1 us each, of 4,096 tokens 13.4 us against 8.4 us).
-constexpr uint64_t kCountsClusterPairs = 1 << 16, kLossClusterTokens = 2048;
+// memset: counts of 2,048 choices 2.7 us against 4.2 us, of 65,536 choices 4.7 us against 5.0 us; BF16 loss of 256 tokens and 256
+// experts 3.9 us against 7.9 us, of 1,536 tokens 7.7 us against 8.3 us, of 1,800 tokens 8.8 us against 8.2 us).  A row of more than
+// 256 experts costs a warp twice as much (512 experts: 768 tokens 8.1 us against 8.2 us, 900 tokens 9.3 us against 8.2 us).
+constexpr uint64_t kCountsClusterPairs = 1 << 16, kLossClusterTokens = 1536;
 constexpr uint32_t kBalMaxBlocks = 592;       // four blocks per SM of a 148-SM device: more warps only repeat the look at the counts
 
 int balance_check(const char* what, const void* z, uint32_t dtype, uint64_t pitch, const void* counts, uint64_t tokens, uint32_t experts) {
@@ -336,7 +337,7 @@ int balance_check(const char* what, const void* z, uint32_t dtype, uint64_t pitc
   return 0;
 }
 
-bool balance_one_cluster(uint64_t tokens, uint32_t experts) { return tokens <= kLossClusterTokens && experts <= 512; }
+bool balance_one_cluster(uint64_t tokens, uint32_t experts) { return experts <= 512 && tokens <= kLossClusterTokens / (experts <= 256 ? 1 : 2); }
 
 uint32_t balance_blocks(uint64_t tokens) {
   const uint64_t b = (tokens + kBalThreads / 32 - 1) / (kBalThreads / 32);
