@@ -674,3 +674,17 @@ def test_results_may_be_modified_in_place():
     loss = balance.balance_loss(flat.clone().requires_grad_(), torch.ones(128, dtype=torch.int32, device="cuda"))
     loss *= 0.5
     loss.backward()
+
+
+@pytest.mark.parametrize("m,n,dtype", [(19000, 40, torch.bfloat16), (20001, 64, torch.float32), (19500, 129, torch.float16)])
+def test_tall_narrow_products_against_64_bits(m, n, dtype):
+    """More row tiles than the device holds at once, and hardly a tile's width of columns."""
+    k = 272
+    g = torch.Generator().manual_seed(m + n)
+    x = (torch.randn(m, k, generator=g) * torch.exp(torch.randn(m, 1, generator=g))).to(dtype)
+    w, ws = make_weight(n, k, n)
+    check_product(dense.fp8_linear(x.cuda(), w, ws), *quantize_definition(x), w, ws)
+    w, ws = make_weight(k, n, n)
+    codes, scale = dense.quantize_rows(x.cuda())
+    check_product(dense.block_scaled_matmul(codes, scale, w, ws, transpose_weight=True, out_dtype=dtype), *quantize_definition(x), w, ws, True)
+    dense.check_status()
