@@ -436,11 +436,13 @@ int netra_moe_sort_static_scratch_launch(const int32_t* topk_ids_i32, int32_t* p
                                          int32_t* offsets_i32, uint32_t rows, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ dense block-scaled FP8 linear map
- * The operation of the compiler's dense contract (compiler/netra_compiler/contracts.py:175-284), at any size.
+ * The operation of the compiler's dense contract (compiler/netra_compiler/contracts.py:175-284), at any size; its K-blocks
+ * are not always added in ascending order (see netra_dense_fp8_matmul_launch).
  * Element types: 0 = BF16, 1 = FP16, 2 = FP32.  Pitches are in elements.  Weights are E4M3 codes [w_rows, w_cols],
  * row-major, with one FP32 scale per 128 x 128 block, [ceil(w_rows/128)] rows of w_scale_pitch >= ceil(w_cols/128).
  * Codes need 16-byte aligned addresses and row pitches; nothing else has an alignment beyond its element.  Sizes are
- * 1..2^26.  Nothing is allocated, synchronised or kept between calls; every call may be captured. */
+ * 1..2^26.  Nothing is allocated, synchronised or kept between calls; every call but
+ * netra_dense_status may be captured. */
 
 /* scale[m,b] = max(amax |x[m, 128 columns of block b]|, 1e-10) * fl(1/448), codes = e4m3_rne_sat(x * fl(1/scale)), all in
  * FP32: the layer's own quantiser.  The scale of (m, b) goes to scale_f32[m * scale_row_stride + b * scale_block_stride].
@@ -450,8 +452,10 @@ int netra_dense_quantize_rows_launch(void* codes_fp8, uint64_t codes_pitch, floa
                                      uint32_t m, uint32_t k, cudaStream_t stream);
 
 /* out[m, n] = sum over K-blocks b of a_scale[m,b] * w_scale[.,.] * sum_{k in b} a[m,k] * w in FP32, one rounding to
- * out_dtype.  The order of the sum depends on the sizes only, so calls repeat bit for bit.  transpose_w = 0: w is [n, k] (a linear layer's weight); 1: w is [k, n] as stored (the gradient to
- * a linear layer's input: w_rows is the reduction).  Scale strides as above. */
+ * out_dtype.  The order of the sum depends on the sizes only, so calls repeat bit for bit: ascending K-blocks, except that few
+ * rows, and few output tiles, add the K-blocks in several parts which are then joined in a fixed order.  transpose_w = 0: w is
+ * [n, k] (a linear layer's weight); 1: w is [k, n] as stored (the gradient to a linear layer's input: w_rows is the reduction).
+ * Scale strides as above. */
 int netra_dense_fp8_matmul_launch(void* out, uint32_t out_dtype, uint64_t out_pitch, const void* a_fp8, uint64_t a_pitch,
                                   const float* a_scale_f32, uint64_t a_scale_row_stride, uint64_t a_scale_block_stride,
                                   const void* w_fp8, uint64_t w_pitch, const float* w_scale_f32, uint64_t w_scale_pitch,

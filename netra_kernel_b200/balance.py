@@ -4,10 +4,12 @@
     loss = balance_loss(logits, counts, token_mask)                   # FP32 scalar, differentiable with respect to logits
 
 With f = counts / sum counts and P_e the mean softmax probability of expert e over the counted tokens,
-``loss = E * sum_e f_e * P_e``: 1 when both are even.  The counts carry no gradient; a data- or expert-parallel program adds
-up the ranks' counts before it calls ``balance_loss``.  Calls enqueue on torch's current stream of the operands' device and may
-be captured in a CUDA graph; results do not depend on the order in which blocks run.  There is no CPU implementation.
-Bad operands raise ValueError, operands that carry a forward-mode tangent NotImplementedError, failures of the C ABI RuntimeError.
+``loss = E * sum_e f_e * P_e``: 1 when both are even; up to ``MAX_EXPERTS`` experts.  The counts carry no gradient; a data- or
+expert-parallel program adds up the ranks' counts before it calls ``balance_loss``.  Calls enqueue on torch's current stream of the
+operands' device and may be captured in a CUDA graph (a backward pass not while an eager graph of one of its leaves, made on
+the default stream, is alive: RuntimeError); results do not depend on the order in which blocks run.  There is no CPU
+implementation.  Bad operands raise ValueError, operands that carry a forward-mode tangent NotImplementedError, failures of the C
+ABI RuntimeError.
 """
 from __future__ import annotations
 

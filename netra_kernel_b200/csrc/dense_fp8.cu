@@ -6,7 +6,8 @@
 //   product    y[m,n] = sum_b  sa[m,b] * sw[n/128,b] * sum_{k in b} a[m,k] w[n,k]
 //   gradient   dx[m,k] = sum_b sg[m,b] * sw[b,k/128] * sum_{n in b} g[m,n] w[n,k]      (w read as it is stored)
 //
-// Any M, N, K: codes need 16-byte row pitches (TMA), everything else is masked.
+// Any M, N, K: codes need 16-byte row pitches (TMA), everything else is masked.  K-blocks are added in ascending order but for few
+// rows (parts by warp) and tiles split over a cluster (parts by CTA), whose parts are joined in a fixed order.
 #include <type_traits>
 
 namespace netra {

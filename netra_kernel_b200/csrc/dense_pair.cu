@@ -4,14 +4,14 @@
 // registers, so three things have to overlap: the tensor core (512 cycles a K-block), the operands (32 KB per CTA and
 // K-block: a pair fetches its weight tile once, half each; one CTA alone would need 48 KB, more than the L2 delivers in that
 // time) and the promotion (128 KB read out of TMEM and 32,768 multiply-adds per CTA).  What bounds it is the chain MMA ->
-// commit -> promotion -> release -> MMA on one accumulator stage: 930 cycles per K-block at two stages, of which the commit
-// across two CTAs alone takes about 400.  Hence:
+// commit -> promotion -> release -> MMA on an accumulator stage: 975 cycles per K-block with the stores (4736 x 4096 x 4096, the
+// busiest pair), and no unit near its limit (57 % of the issue slots; half of shared memory, a quarter of the L2).  Hence:
 //   * sixteen promotion warps, four per scheduler, hide latencies that eight cannot; a thread keeps 64 columns of its row;
 //   * a K-block is multiplied and handed over in two halves of 128 columns, each with its own barriers (140 -> 133 us at
 //     16384 x 4096 x 2048), by two issuing threads that take alternate K-blocks (151 -> 137 us);
 //   * the scales go through shared memory, four K-blocks ahead: loaded by the promotion warps themselves, one K-block ahead,
 //     they were what the loop waited for (172 -> 151 us).
-// 16384 x 4096 x 2048: 133 us = 2.06 PFLOP/s in a burst, 157 us back to back for seconds (1,000 W cap, 1.59 GHz).
+// 16384 x 4096 x 2048: 130-133 us = 2.1 PFLOP/s in a burst, 157 us back to back for seconds (1,000 W cap, 1.59 GHz).
 //
 //   warp 0: TMA producer (each CTA its own 128 rows and its own 128 weight rows; both report to the leader's barrier)
 //   warps 1 and 3: MMA issuers (leader CTA) or relays of the peer's releases (warp 1 also owns TMEM), warp 2: scales,
@@ -240,7 +240,7 @@ netra_dense_fp8_pair_sm100(const __grid_constant__ CUtensorMap tm_a, const __gri
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairRegsHigh));
     const int wg = (warp - 4) >> 2, quad = warp & 3;            // 64 columns and 32 rows of this warp
     const uint32_t tile = smem_u32(staging) + (uint32_t)(warp - 4) * 4096u, my_row = tile + (uint32_t)lane * 128u;
-    // This loop is paced by the instructions its sixteen warps issue (four per scheduler), so what can be carried from one
+    // Every instruction here lengthens the chain above (a leaner loop: 673 -> 618 ns a K-block), so what can be carried from one
     // K-block to the next is carried: the barrier's address and phase, the scales' slot (four stages and two phases make the
     // eight slots), the TMEM column of the accumulator stage.
     const uint32_t bar0 = smem_u32(&done_bar[wg >> 1]);

@@ -1,6 +1,7 @@
 """The dense block-scaled FP8 linear map of the compiler's dense contract, for the projections around the routed-MoE layer:
-E4M3 weights with one FP32 scale per 128 x 128 block (a frozen checkpoint), activations quantised per token and 128
-columns by the layer's own quantiser, FP32 accumulation, one rounding to the activations' type.
+E4M3 weights with one FP32 scale per ``BLOCK`` x ``BLOCK`` = 128 x 128 block (a frozen checkpoint), activations quantised per token
+and 128 columns by the layer's own quantiser, FP32 accumulation, one rounding to the activations' type.  Sums repeat bit for bit;
+K-blocks are added in ascending order except for few rows or few output tiles, which join several parts in a fixed order.
 
     codes, scale = quantize_rows(x)                                   # x [..., K] -> E4M3 [M, K], FP32 [M, ceil(K/128)]
     y = block_scaled_matmul(codes, scale, weight, weight_scale)       # [M, N]
@@ -41,8 +42,8 @@ def block_scaled_matmul(a: torch.Tensor, a_scale: torch.Tensor, weight: torch.Te
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a`` [M, K] E4M3 with scales [M, ceil(K/128)] times a block-scaled weight: ``a @ weight.T`` [M, N] for ``weight``
     [N, K], or with ``transpose_weight`` ``a`` [M, N] times ``weight`` as it is stored -> [M, K].  ``weight_scale`` is
-    [ceil(N/128), ceil(K/128)] either way.  ``out`` (row-major, no memory of an operand) takes the result in its own type.  The product carries
-    no gradient and refuses operands that require one, unless gradients are off."""
+    [ceil(N/128), ceil(K/128)] either way.  ``out`` (row-major, no memory of an operand) takes the result in its own type.  The
+    product carries no gradient and refuses operands that require one, unless gradients are off."""
     return _ext.block_scaled_matmul(a, a_scale, weight, weight_scale, transpose_weight, out_dtype, out)
 
 
@@ -52,7 +53,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
     Differentiable with respect to x: the incoming gradient's rows are quantised the same way and multiplied by the weight as
     it is stored (``block_scaled_matmul(..., transpose_weight=True)``); the rounding of x to E4M3 passes gradients unchanged.
-    The weight is frozen.  The gradient cannot be differentiated again with respect to the incoming one: that raises RuntimeError."""
+    The weight is frozen.  The gradient cannot be differentiated again with respect to the incoming one: that raises
+    RuntimeError."""
     return _ext.fp8_linear(x, weight, weight_scale)
 
 
